@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define TTC_ABI_VERSION 7
+#define TTC_ABI_VERSION 8
 
 #define TTC_DTYPE_F32 0
 #define TTC_DTYPE_BF16 1
@@ -280,6 +280,92 @@ int ttc_prologue_bwd(const void* Z, int64_t N, int nh, int d, int du, int rB, in
                      const void* g_A_diag, const void* g_R_inv, const void* g_coeff_Qf,
                      const void* g_lgA, const void* g_lgB, const void* g_lgQ, const void* g_h0,
                      const void* g_coeff_B, const void* g_coeff_Q, void* dZ, void* stream);
+
+/*
+ * Sequence operators beside the layer: attention with a fixed decay for each head, rotary
+ * positions and the group norm of a token's heads.  No counterpart in the reference, whose layer
+ * mixes no tokens; a language model puts such a memory next to it.
+ *
+ * Attention with a decay: for every sequence and head h, gamma = exp(log_gamma[h]),
+ *   S_t = gamma S_{t-1} + k_t^T v_t,   o_t = scale q_t S_t,
+ * S [dk, dv] in fp32, S_{-1} = initial_state or 0.  q, k [.., Hk, dk] and v [.., H, dv] in the
+ * activation dtype, H a multiple of Hk (head h reads key head h / (H / Hk)); dk, dv multiples
+ * of 8 from 8 to 128 (TTC_ERR_UNSUPPORTED otherwise).  log_gamma [H] float32; -inf is a head without memory.
+ *
+ * Sequences: n_seq sequences of T tokens (q [n_seq, T, Hk, dk], ...), or, with cu_seqlens
+ * (device int32 [n_seq + 1], non-decreasing), packed: tokens cu_seqlens[i] .. cu_seqlens[i + 1] - 1
+ * of one row of T tokens.  Offsets are cut to [0, T] before use; rows of o and of the gradients
+ * behind the last sequence are zeros.  Empty sequences are allowed (their last state is their
+ * first).
+ * strides (host memory): batch, token and head strides of q, then k, then v, in elements, each a
+ * multiple of 16 bytes; the head dims are contiguous and every pointer is 16-byte aligned.
+ * Outputs, g_o and states are contiguous: o, g_o, d_v [.., H, dv], d_q, d_k [.., Hk, dk], states
+ * [n_seq, H, dk, dv] float32.  initial_state, final_state, g_final_state and
+ * d_initial_state may be NULL.
+ * workspace: ttc_decay_attn_workspace(...) bytes (T, n_seq, packed as above; minus an error code
+ * for bad sizes), 16-byte aligned, not shared by calls that may overlap; its contents need not be kept
+ * between the forward and the backward.
+ */
+int64_t ttc_decay_attn_workspace(int64_t T, int n_seq, int packed, int H, int Hk, int dk, int dv, int dtype,
+                                 int backward);
+int ttc_decay_attn_fwd(const void* q, const void* k, const void* v, const int64_t* strides,
+                       const float* log_gamma, float scale, const float* initial_state,
+                       const int* cu_seqlens, int64_t T, int n_seq, int H, int Hk, int dk, int dv, int dtype,
+                       void* o, float* final_state, void* workspace, int64_t workspace_bytes, void* stream);
+/* Gradients of o (g_o) and of the last state (g_final_state, NULL = 0) to q, k, v and the first
+ * state; those of shared key heads are summed over their heads in fp32, in order. */
+int ttc_decay_attn_bwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* g_o,
+                       const float* log_gamma, float scale, const float* initial_state,
+                       const float* g_final_state, const int* cu_seqlens, int64_t T, int n_seq, int H, int Hk,
+                       int dk, int dv, int dtype, void* d_q, void* d_k, void* d_v, float* d_initial_state,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+/* One token for each of B rows: row b advances state number slots[b] (b where slots is NULL) of
+ * n_slots states, each [H, dk, dv] float32 contiguous, slot_stride elements apart and 16-byte aligned, in
+ * place, and writes o [B, H, dv].  Rows of the same slot are taken as consecutive tokens in the
+ * order of the rows.  A row whose slot is outside [0, n_slots) is padding: its o is zeros and no
+ * state changes.  q, k [B, Hk, dk], v [B, H, dv]; strides (host): batch and head stride of q, k, v,
+ * in elements, any values. */
+int ttc_decay_attn_step(const void* q, const void* k, const void* v, const int64_t* strides,
+                        const float* log_gamma, float scale, float* state, int64_t slot_stride,
+                        const int* slots, int B, int n_slots, int H, int Hk, int dk, int dv, int dtype,
+                        void* o, void* stream);
+
+/*
+ * Rotary positions of q [B, T, Hq, D] and k [B, T, Hk, D] (Hk = 0: q alone) in one launch: pair p
+ * of the first 2 half values of each head, (p, p + half) or, interleaved, (2p, 2p + 1), turns by
+ * positions[b, t] * inv_freq[p] and is multiplied by `magnitude`; the others are copied.  inverse
+ * turns back (the backward: it multiplies by `magnitude` too).  positions: int64 (pos64) or int32,
+ * with their batch and token strides (0 to share them); inv_freq [half] float64, both on the
+ * device.  Angles are formed and reduced in 64 bits.  Strides (host): batch, token, head, in elements; outputs are
+ * contiguous.  D <= 512.
+ */
+int ttc_rotary(const void* q, const int64_t* q_strides, int Hq, const void* k, const int64_t* k_strides, int Hk,
+               const void* positions, const int64_t* pos_strides, int pos64, const double* inv_freq,
+               int64_t B, int64_t T, int D, int half, int interleaved, int inverse, float magnitude, int dtype,
+               void* q_out, void* k_out, void* stream);
+
+/* Activations of ttc_group_norm_*: the identity, u sigmoid(u), u Phi(u). */
+#define TTC_ACT_NONE 0
+#define TTC_ACT_SILU 1
+#define TTC_ACT_GELU 2
+
+/*
+ * Group norm over the channels of each row: x [rows, groups * n] (channels contiguous, rows
+ * x_stride elements apart), xhat = (x - mean) / sqrt(var + eps) over each group of n <= 1024
+ * channels in fp32, z = xhat weight + bias (either may be NULL), and y [rows, groups * n] = act(z)
+ * or, with a gate (as x, its own row stride), z act(gate).  weight, bias: float32 where
+ * param_f32, else the activation dtype.
+ * Backward, from g (contiguous): dx, dgate, dweight, dbias, each may be NULL; the sums over the rows run in fp32
+ * in a fixed order.  workspace: ttc_group_norm_workspace bytes, needed for dweight or dbias.
+ */
+int64_t ttc_group_norm_workspace(int64_t rows, int groups, int n, int dtype);
+int ttc_group_norm_fwd(const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,
+                       const void* weight, const void* bias, int param_f32, int64_t rows, int groups, int n,
+                       int act, float eps, int dtype, void* y, void* stream);
+int ttc_group_norm_bwd(const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,
+                       const void* weight, const void* bias, int param_f32, const void* g, int64_t rows,
+                       int groups, int n, int act, float eps, int dtype, void* dx, void* dgate, void* dweight,
+                       void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

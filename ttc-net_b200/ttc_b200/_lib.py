@@ -13,7 +13,7 @@ import threading
 # compiled with tuning macros by `build.py --out PATH -D NAME=VALUE`).
 LIB_PATH = os.environ.get("TTC_B200_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)),
                                                           "libttc_b200.so")
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
@@ -33,11 +33,17 @@ STATUS_COPY_TIMEOUT = 64
 
 FLAG_INV_GUARD = 1
 
+ACT_NONE = 0
+ACT_SILU = 1
+ACT_GELU = 2
+
 # Every symbol include/ttc_b200.h declares, with (restype, argtypes).
 _P = ctypes.c_void_p
 _FP = ctypes.c_void_p      # float* passed as a raw address
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
+_F = ctypes.c_float
+_SP = ctypes.POINTER(ctypes.c_int64)  # strides, in host memory
 SIGNATURES = {
     "ttc_abi_version": (_I, []),
     "ttc_supported": (_I, [_I, _I]),
@@ -61,6 +67,16 @@ SIGNATURES = {
     "ttc_rownorm_bwd": (_I, [_P, _P, _I64, _I, _I, _P, _P]),
     "ttc_prologue_fwd": (_I, [_P, _I64] + [_I] * 6 + [_P] * 9 + [_P, _P]),
     "ttc_prologue_bwd": (_I, [_P, _I64] + [_I] * 6 + [_P] * 9 + [_P, _P]),
+    "ttc_decay_attn_workspace": (_I64, [_I64] + [_I] * 8),
+    "ttc_decay_attn_fwd": (_I, [_P] * 3 + [_SP, _FP, _F, _FP, _P, _I64] + [_I] * 6 + [_P, _FP, _P, _I64, _P]),
+    "ttc_decay_attn_bwd": (_I, [_P] * 3 + [_SP, _P, _FP, _F, _FP, _FP, _P, _I64] + [_I] * 6
+                           + [_P] * 3 + [_FP, _P, _I64, _P]),
+    "ttc_decay_attn_step": (_I, [_P] * 3 + [_SP, _FP, _F, _FP, _I64, _P] + [_I] * 7 + [_P, _P]),
+    "ttc_rotary": (_I, [_P, _SP, _I, _P, _SP, _I, _P, _SP, _I, _P, _I64, _I64] + [_I] * 4 + [_F, _I] + [_P] * 3),
+    "ttc_group_norm_workspace": (_I64, [_I64, _I, _I, _I]),
+    "ttc_group_norm_fwd": (_I, [_P, _I64, _P, _I64, _P, _P, _I, _I64, _I, _I, _I, _F, _I, _P, _P]),
+    "ttc_group_norm_bwd": (_I, [_P, _I64, _P, _I64, _P, _P, _I, _P, _I64, _I, _I, _I, _F, _I]
+                           + [_P] * 5 + [_I64, _P]),
 }
 
 _lib = None

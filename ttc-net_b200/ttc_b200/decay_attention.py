@@ -1,0 +1,190 @@
+"""Attention with a fixed decay for each head: the memory over tokens that stands beside the
+TTC layer, which mixes none.
+
+    S_t = gamma_h S_{t-1} + k_t^T v_t,   o_t = scale q_t S_t,   gamma_h = exp(log_gamma[h])
+
+``decay_attention`` takes whole sequences (prompts and training; ``ttc_decay_attn_fwd`` / ``_bwd``,
+blocks of 64 tokens on the tensor cores, the state in fp32 registers), ``decay_attention_step`` one token
+for each row over a cache of states (``ttc_decay_attn_step``).  No counterpart in the reference; no
+fallback: without the CUDA library these raise.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .solver import _DTYPES, _aligned, _launch, _ptr
+
+
+def _workspace(nbytes: int, dev) -> torch.Tensor | None:
+    """Scratch memory of one call, on the call's stream."""
+    if nbytes < 0:
+        _lib.check(-nbytes)
+    return torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+
+
+def _operand(t: torch.Tensor) -> torch.Tensor:
+    """t itself if its head dim is contiguous and its rows start on 16-byte boundaries (a slice of
+    a fused projection, an expanded tensor), else a contiguous copy."""
+    es = t.element_size()
+    ok = t.stride(-1) == 1 and all(n == 1 or s * es % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()))
+    return _aligned(t if ok else t.contiguous())
+
+
+def _strides(*tensors):
+    flat = [0 if n == 1 else s for t in tensors for n, s in zip(t.shape[:-1], t.stride())]
+    return (ctypes.c_int64 * len(flat))(*flat)
+
+
+def _check_qkv(name, q, k, v, log_gamma, lead):
+    """Types, devices and shapes of q, k [*lead, Hk, dk], v [*lead, H, dv], log_gamma [H]."""
+    for t, n in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dtype not in _DTYPES:
+            raise TypeError(f"ttc_b200 {name} supports float32 and bfloat16, got {t.dtype} for {n}")
+        if t.dim() != lead + 2:
+            raise ValueError(f"ttc_b200 {name}: {n} must have {lead + 2} dimensions, got {tuple(t.shape)}")
+    if not q.dtype == k.dtype == v.dtype:
+        raise TypeError(f"ttc_b200 {name}: q, k and v must have one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if q.shape != k.shape or q.shape[:lead] != v.shape[:lead]:
+        raise ValueError(f"ttc_b200 {name}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
+    Hk, dk = q.shape[lead:]
+    H, dv = v.shape[lead:]
+    if Hk < 1 or H % Hk:
+        raise ValueError(f"ttc_b200 {name}: {H} value heads are not a multiple of {Hk} key heads")
+    if tuple(log_gamma.shape) != (H,) or not log_gamma.dtype.is_floating_point:
+        raise ValueError(f"ttc_b200 {name}: log_gamma must be [{H}] floating point, got {tuple(log_gamma.shape)}")
+    if torch.is_grad_enabled() and log_gamma.requires_grad:
+        raise ValueError(f"ttc_b200 {name}: the decays are fixed, log_gamma must not require a gradient")
+    return H, Hk, dk, dv
+
+
+def _check_device(name, dev, **tensors):
+    for n, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"ttc_b200 {name}: {n} is on {t.device}, q on {dev}")
+    if dev.type != "cuda":
+        raise ValueError(f"ttc_b200 {name} needs CUDA tensors (there is no CPU path)")
+
+
+class DecayAttentionFunction(torch.autograd.Function):
+    """(q, k, v, initial_state) -> (o, last state or None)."""
+
+    @staticmethod
+    @torch.amp.custom_fwd(device_type="cuda")
+    def forward(ctx, q, k, v, log_gamma, scale, initial_state, cu_seqlens, want_state):
+        dev = q.device
+        q, k, v = _operand(q), _operand(k), _operand(v)
+        B, T, Hk, dk = q.shape
+        H, dv = v.shape[2:]
+        packed = cu_seqlens is not None
+        n_seq = cu_seqlens.numel() - 1 if packed else B
+        lib = _lib.load()
+        dims = (T, n_seq, H, Hk, dk, dv, _DTYPES[q.dtype])
+        with torch.cuda.device(dev):
+            o = torch.empty(B, T, H, dv, device=dev, dtype=q.dtype)
+            state = torch.empty(n_seq, H, dk, dv, device=dev) if want_state else None
+            nbytes = lib.ttc_decay_attn_workspace(T, n_seq, packed, *dims[2:], 0)
+            ws = _workspace(nbytes, dev)
+            _launch("ttc_decay_attn_fwd", dev, lib.ttc_decay_attn_fwd, _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v),
+                    _ptr(log_gamma), scale, _ptr(initial_state), _ptr(cu_seqlens), *dims, _ptr(o), _ptr(state),
+                    _ptr(ws), nbytes)
+        ctx.save_for_backward(q, k, v, log_gamma, initial_state, cu_seqlens)
+        ctx.dims, ctx.scale = dims, scale
+        return o, state
+
+    @staticmethod
+    @torch.amp.custom_bwd(device_type="cuda")
+    @once_differentiable
+    def backward(ctx, g_o, g_state):
+        q, k, v, log_gamma, initial_state, cu_seqlens = ctx.saved_tensors
+        dev = q.device
+        packed = cu_seqlens is not None
+        g_o = torch.zeros(v.shape, device=dev, dtype=v.dtype) if g_o is None else _aligned(g_o.to(v.dtype).contiguous())
+        g_state = None if g_state is None else g_state.float().contiguous()
+        lib = _lib.load()
+        T, n_seq = ctx.dims[:2]
+        with torch.cuda.device(dev):
+            d_q, d_k, d_v = (torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k, v))
+            d_s = None
+            if initial_state is not None and ctx.needs_input_grad[5]:
+                d_s = torch.empty(initial_state.shape, device=dev)
+            nbytes = lib.ttc_decay_attn_workspace(T, n_seq, packed, *ctx.dims[2:], 1)
+            ws = _workspace(nbytes, dev)
+            _launch("ttc_decay_attn_bwd", dev, lib.ttc_decay_attn_bwd, _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v),
+                    _ptr(g_o), _ptr(log_gamma), ctx.scale, _ptr(initial_state), _ptr(g_state), _ptr(cu_seqlens),
+                    *ctx.dims, _ptr(d_q), _ptr(d_k), _ptr(d_v), _ptr(d_s), _ptr(ws), nbytes)
+        return d_q, d_k, d_v, None, None, d_s, None, None
+
+
+def decay_attention(q, k, v, log_gamma, scale: float | None = None, initial_state=None, return_state: bool = False,
+                    cu_seqlens=None):
+    """o [B, T, H, dv] for q, k [B, T, Hk, dk] and v [B, T, H, dv] (float32 or bfloat16; H a multiple of
+    Hk, head h reads key head h // (H // Hk); dk, dv multiples of 8 up to 128), log_gamma [H] the logarithm
+    of each head's decay (fixed: no gradient; -inf is no memory).  ``scale`` defaults to
+    dk ** -0.5.  Differentiable in q, k, v and ``initial_state`` [B, H, dk, dv] float32.
+
+    ``return_state``: (o, state), the states behind the last tokens, float32, from which
+    ``decay_attention_step`` or another call goes on.
+
+    ``cu_seqlens`` (int32 [n + 1] on the device, from 0, non-decreasing): packed sequences, B = 1 and
+    sequence i the tokens cu_seqlens[i] .. cu_seqlens[i + 1] - 1; states are [n, H, dk, dv].  Rows
+    behind the last sequence get zeros.  Offsets past the row are cut to it.
+
+    A token's output depends on no later token, whatever that holds.  Any strides with a contiguous
+    head dim are read in place if rows start on 16-byte boundaries."""
+    name = "decay_attention"
+    H, Hk, dk, dv = _check_qkv(name, q, k, v, log_gamma, 2)
+    n_seq = q.shape[0]
+    if cu_seqlens is not None:
+        if q.shape[0] != 1:
+            raise ValueError(f"ttc_b200 {name}: packed sequences need a batch of 1, got {q.shape[0]}")
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
+            raise ValueError(f"ttc_b200 {name}: cu_seqlens must be int32 [n + 1] with n >= 1")
+        n_seq = cu_seqlens.numel() - 1
+    if initial_state is not None and (initial_state.dtype != torch.float32
+                                      or tuple(initial_state.shape) != (n_seq, H, dk, dv)):
+        raise ValueError(f"ttc_b200 {name}: initial_state must be float32 [{n_seq},{H},{dk},{dv}], got "
+                         f"{initial_state.dtype} {tuple(initial_state.shape)}")
+    _check_device(name, q.device, k=k, v=v, log_gamma=log_gamma, initial_state=initial_state, cu_seqlens=cu_seqlens)
+    o, state = DecayAttentionFunction.apply(
+        q, k, v, log_gamma.detach().float().contiguous(), dk ** -0.5 if scale is None else float(scale),
+        None if initial_state is None else initial_state.contiguous(),
+        None if cu_seqlens is None else cu_seqlens.contiguous(), bool(return_state))
+    return (o, state) if return_state else o
+
+
+def decay_attention_step(q, k, v, log_gamma, state, slots=None, scale: float | None = None) -> torch.Tensor:
+    """One token for each row: q, k [B, Hk, dk], v [B, H, dv] -> o [B, H, dv].  ``state`` [n, H, dk, dv]
+    float32 is the cache of states, advanced in place; row b goes on from state ``slots[b]`` (int32 on the
+    device; b without ``slots``).  Rows of one slot are consecutive tokens in the rows' order; a row whose slot
+    is outside [0, n) is padding, its output is zeros.  Records no gradient."""
+    name = "decay_attention_step"
+    H, Hk, dk, dv = _check_qkv(name, q, k, v, log_gamma, 1)
+    if state.dtype != torch.float32 or state.dim() != 4 or tuple(state.shape[1:]) != (H, dk, dv):
+        raise ValueError(f"ttc_b200 {name}: state must be float32 [n,{H},{dk},{dv}], got "
+                         f"{state.dtype} {tuple(state.shape)}")
+    B, n = q.shape[0], state.shape[0]
+    if not state[:1].is_contiguous() or state.data_ptr() % 16 or (n > 1 and (state.stride(0) % 4
+                                                                             or state.stride(0) < H * dk * dv)):
+        raise ValueError(f"ttc_b200 {name}: each state must be contiguous and start on a 16-byte boundary")
+    if slots is not None and (slots.dtype != torch.int32 or tuple(slots.shape) != (B,)):
+        raise ValueError(f"ttc_b200 {name}: slots must be int32 [{B}], got {slots.dtype} {tuple(slots.shape)}")
+    if slots is None and n < B:
+        raise ValueError(f"ttc_b200 {name}: {B} rows and {n} states")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
+        raise ValueError(f"ttc_b200 {name} records no gradient: call it under torch.no_grad()")
+    dev = q.device
+    _check_device(name, dev, k=k, v=v, log_gamma=log_gamma, state=state, slots=slots)
+    q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
+    log_gamma = log_gamma.detach().float().contiguous()
+    slots = None if slots is None else slots.contiguous()
+    with torch.cuda.device(dev):
+        o = torch.empty(B, H, dv, device=dev, dtype=q.dtype)
+        _launch("ttc_decay_attn_step", dev, _lib.load().ttc_decay_attn_step, _ptr(q), _ptr(k), _ptr(v),
+                _strides(q, k, v), _ptr(log_gamma), dk ** -0.5 if scale is None else float(scale), _ptr(state),
+                state.stride(0) if n > 1 else H * dk * dv, _ptr(slots), B, n, H, Hk, dk, dv, _DTYPES[q.dtype], _ptr(o))
+    torch.autograd.graph.increment_version(state)
+    return o

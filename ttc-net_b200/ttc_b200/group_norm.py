@@ -1,0 +1,95 @@
+"""Group norm over the channels of each token, with an activation or a gate: the norm of the
+heads' outputs behind ``decay_attention``, beside the l2norm of the TTC layer's epilogue
+(``epilogue.py``).  One CUDA kernel forward (``ttc_group_norm_fwd``), one backward and a small sum over
+rows for the parameters (``ttc_group_norm_bwd``, which recomputes the statistics).  No counterpart in the reference;
+no fallback: without the CUDA library this raises.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .decay_attention import _workspace
+from .solver import _DTYPES, _launch, _ptr
+
+_ACTS = {"none": _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}
+
+
+def _rows(t, C):
+    """t as [rows, C] with contiguous channels, a view where its strides allow."""
+    t = t.reshape(-1, C)
+    return t if t.stride(1) == 1 or C == 1 else t.contiguous()
+
+
+class GroupNormFunction(torch.autograd.Function):
+    """(x, weight, bias, gate) -> y, all but x may be None."""
+
+    @staticmethod
+    @torch.amp.custom_fwd(device_type="cuda")
+    def forward(ctx, x, weight, bias, gate, groups, act, eps):
+        shape, C, dev = x.shape, x.shape[-1], x.device
+        x2, gate2 = _rows(x, C), None if gate is None else _rows(gate, C)
+        weight, bias = (None if p is None else p.contiguous() for p in (weight, bias))
+        some = weight if weight is not None else bias
+        ctx.dims = (x2.shape[0], groups, C // groups, act, eps, _DTYPES[x.dtype])
+        ctx.param_f32 = int(some is not None and some.dtype == torch.float32)
+        ctx.shape = shape
+        with torch.cuda.device(dev):
+            y = torch.empty(shape, device=dev, dtype=x.dtype)
+            _launch("ttc_group_norm_fwd", dev, _lib.load().ttc_group_norm_fwd, _ptr(x2), x2.stride(0), _ptr(gate2),
+                    0 if gate2 is None else gate2.stride(0), _ptr(weight), _ptr(bias), ctx.param_f32, *ctx.dims, _ptr(y))
+        ctx.save_for_backward(x2, weight, bias, gate2)
+        return y
+
+    @staticmethod
+    @torch.amp.custom_bwd(device_type="cuda")
+    @once_differentiable
+    def backward(ctx, g):
+        x, weight, bias, gate = ctx.saved_tensors
+        dev, dtype = x.device, x.dtype
+        g = g.to(dtype).contiguous()
+        lib = _lib.load()
+        with torch.cuda.device(dev):
+            def like(on, t, shape):
+                return torch.empty(shape, device=dev, dtype=t.dtype) if on and t is not None else None
+
+            needs = ctx.needs_input_grad
+            dx = like(needs[0], x, ctx.shape)
+            dw, db = (like(needs[i], p, p.shape if p is not None else None) for i, p in ((1, weight), (2, bias)))
+            dgate = like(needs[3], gate, ctx.shape)
+            rows, groups, n, act, eps, code = ctx.dims
+            nbytes = lib.ttc_group_norm_workspace(rows, groups, n, code) if dw is not None or db is not None else 0
+            ws = _workspace(nbytes, dev)
+            _launch("ttc_group_norm_bwd", dev, lib.ttc_group_norm_bwd, _ptr(x), x.stride(0), _ptr(gate),
+                    0 if gate is None else gate.stride(0), _ptr(weight), _ptr(bias), ctx.param_f32, _ptr(g), rows,
+                    groups, n, act, eps, code, _ptr(dx), _ptr(dgate), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
+        return dx, dw, db, dgate, None, None, None
+
+
+def group_norm(x, num_groups: int, weight=None, bias=None, gate=None, activation: str = "none", eps: float = 1e-5):
+    """y, shaped like x [..., C] (float32 or bfloat16): the C channels of each row in ``num_groups`` groups (heads) of
+    at most 1024, each to mean 0 and variance 1 (fp32), times ``weight`` [C] plus ``bias`` [C] (x's dtype
+    or float32), then ``activation`` ("none", "silu" or "gelu", the exact one).  With ``gate`` (x's
+    shape) the activation is of the gate and multiplies: norm(x) * act(gate).  Rows do not mix, so a
+    token's result does not depend on other tokens.  Differentiable in x, weight, bias and gate."""
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"ttc_b200 group_norm supports float32 and bfloat16, got {x.dtype}")
+    if activation not in _ACTS:
+        raise ValueError(f"ttc_b200 group_norm: unknown activation {activation!r}")
+    if x.dim() < 1 or num_groups < 1 or x.shape[-1] < 1 or x.shape[-1] % num_groups:
+        raise ValueError(f"ttc_b200 group_norm: {tuple(x.shape)} channels do not divide into {num_groups} groups")
+    C = x.shape[-1]
+    if gate is not None and (gate.shape != x.shape or gate.dtype != x.dtype):
+        raise ValueError(f"ttc_b200 group_norm: gate must be {x.dtype} {tuple(x.shape)}, got "
+                         f"{gate.dtype} {tuple(gate.shape)}")
+    params = [p for p in (weight, bias) if p is not None]
+    for p in params:
+        if tuple(p.shape) != (C,) or p.dtype not in (x.dtype, torch.float32) or p.dtype != params[0].dtype:
+            raise ValueError(f"ttc_b200 group_norm: weight and bias must be [{C}] in {x.dtype} or both float32")
+    for t, n in ((weight, "weight"), (bias, "bias"), (gate, "gate")):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"ttc_b200 group_norm: {n} is on {t.device}, x on {x.device}")
+    if not x.is_cuda:
+        raise ValueError("ttc_b200 group_norm needs CUDA tensors (there is no CPU path)")
+    return GroupNormFunction.apply(x, weight, bias, gate, int(num_groups), _ACTS[activation], float(eps))
