@@ -305,20 +305,22 @@ int ttc_prologue_bwd(const void* Z, int64_t N, int nh, int d, int du, int rB, in
  * workspace: ttc_decay_attn_workspace(...) bytes (T, n_seq, packed as above; minus an error code
  * for bad sizes), 16-byte aligned, not shared by calls that may overlap; its contents need not be kept
  * between the forward and the backward.
+ * status (device or mapped host int, may be NULL): TTC_STATUS_MMA_TIMEOUT is OR-ed in if a wait
+ * inside a kernel ran out (its outputs are then not valid).
  */
 int64_t ttc_decay_attn_workspace(int64_t T, int n_seq, int packed, int H, int Hk, int dk, int dv, int dtype,
                                  int backward);
 int ttc_decay_attn_fwd(const void* q, const void* k, const void* v, const int64_t* strides,
                        const float* log_gamma, float scale, const float* initial_state,
                        const int* cu_seqlens, int64_t T, int n_seq, int H, int Hk, int dk, int dv, int dtype,
-                       void* o, float* final_state, void* workspace, int64_t workspace_bytes, void* stream);
+                       void* o, float* final_state, void* workspace, int64_t workspace_bytes, int* status, void* stream);
 /* Gradients of o (g_o) and of the last state (g_final_state, NULL = 0) to q, k, v and the first
  * state; those of shared key heads are summed over their heads in fp32, in order. */
 int ttc_decay_attn_bwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* g_o,
                        const float* log_gamma, float scale, const float* initial_state,
                        const float* g_final_state, const int* cu_seqlens, int64_t T, int n_seq, int H, int Hk,
                        int dk, int dv, int dtype, void* d_q, void* d_k, void* d_v, float* d_initial_state,
-                       void* workspace, int64_t workspace_bytes, void* stream);
+                       void* workspace, int64_t workspace_bytes, int* status, void* stream);
 /* One token for each of B rows: row b advances state number slots[b] (b where slots is NULL) of
  * n_slots states, each [H, dk, dv] float32 contiguous, slot_stride elements apart and 16-byte aligned, in
  * place, and writes o [B, H, dv].  Rows of the same slot are taken as consecutive tokens in the

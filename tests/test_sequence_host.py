@@ -27,11 +27,11 @@ def test_decay_attention_abi_rejects_bad_arguments(lib):
     def fwd(q=P, o=P, fin=None, T=8, n=1, H=4, Hk=2, dk=16, dv=16, dtype=0, strides=_i64(*[64] * 9), cu=None, ws=None,
             nbytes=0):
         return lib.ttc_decay_attn_fwd(q, P, P, strides, P, 1.0, None, cu, T, n, H, Hk, dk, dv, dtype, o, fin, ws, nbytes,
-                                      None)
+                                      None, None)
 
     def bwd(g=P, dq=P, T=8, n=1, H=4, Hk=4, nbytes=0):
         return lib.ttc_decay_attn_bwd(P, P, P, _i64(*[64] * 9), g, P, 1.0, None, None, None, T, n, H, Hk, 16, 16, 0, dq, P, P,
-                                      None, None, nbytes, None)
+                                      None, None, nbytes, None, None)
 
     assert fwd(T=-1) == _lib.ERR_INVALID
     assert fwd(T=1 << 31) == _lib.ERR_INVALID

@@ -208,6 +208,9 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// bf16 heads run on tcgen05 (decay_attn_tc.cuh) from this width on.
+bool use_tc(int dtype, int dk, int dv) { return dtype == TTC_DTYPE_BF16 && std::max(dk, dv) > 32; }
+
 struct Plan {
   int seg_len, n_seg, items;
 };
@@ -216,7 +219,7 @@ struct Plan {
 // the sequences are cut into segments of about equal shares of all tokens for two CTAs an SM.  A
 // segment's state costs a second pass over k and v and four trips of its elements through memory, so a
 // segment has at least 512 tokens.
-Plan plan(int64_t T, int n_seq, bool packed, int H, int passes) {
+Plan plan(int64_t T, int n_seq, bool packed, int H, int passes, bool tc) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
@@ -224,10 +227,11 @@ Plan plan(int64_t T, int n_seq, bool packed, int H, int passes) {
     sms = 148;
   }
   const int64_t rows = static_cast<int64_t>(n_seq) * H * passes;
+  const int64_t slots = (tc ? 1 : 2) * sms;
   int64_t len = T;
-  if (rows < 2 * sms) {
+  if (rows < slots) {
     const int64_t all = (packed ? T : T * n_seq) * H * passes;
-    len = std::max<int64_t>(512, (all + 2 * sms - 1) / (2 * sms));
+    len = std::max<int64_t>(512, (all + slots - 1) / slots);
     if (!packed && len < T) len = (T + (T + len - 1) / len - 1) / ((T + len - 1) / len);  // segments of one length
   }
   Plan p;
@@ -268,9 +272,12 @@ int64_t state_bytes(const Plan& p, int64_t T, int H, int dk, int dv, int passes)
   return segmented(p, T) ? static_cast<int64_t>(p.items) * H * dk * dv * 4 * passes : 0;
 }
 
-int run_passes(Args& A, const Pass* pass, int n, int dtype, bool seg, cudaStream_t st) {
-  auto go = dtype == TTC_DTYPE_BF16 ? launch_bf16 : launch_f32;
-  const auto same = [](const Pass& x, const Pass& y) {
+int run_passes(Args& A, const Pass* pass, int n, int dtype, bool seg, bool tc, int* status, cudaStream_t st) {
+  const auto go = [&](const Args& a, int m, bool state_only) {
+    return dtype == TTC_DTYPE_BF16 ? launch_bf16(a, m, state_only, tc, status, st) : launch_f32(a, m, state_only, st);
+  };
+  const auto same = [tc](const Pass& x, const Pass& y) {
+    if (tc) return (x.kd > 64) == (y.kd > 64) && (x.vd > 64) == (y.vd > 64);
     return width_class(x.kd) == width_class(y.kd) && width_class(x.vd) == width_class(y.vd);
   };
   for (int phase = seg ? 0 : 2; phase < 3; ++phase) {
@@ -290,7 +297,7 @@ int run_passes(Args& A, const Pass* pass, int n, int dtype, bool seg, cudaStream
           A.pass[m++] = pass[j];
           done[j] = true;
         }
-      if (int rc = go(A, m, phase == 0, st)) return rc;
+      if (int rc = go(A, m, phase == 0)) return rc;
     }
   }
   return TTC_OK;
@@ -307,7 +314,7 @@ extern "C" int64_t ttc_decay_attn_workspace(int64_t T, int n_seq, int packed, in
   if (int rc = da::check(T, n_seq, H, Hk, dk, dv, dtype)) return -rc;
   if (n_seq == 0) return 0;
   const int passes = backward ? 3 : 1;
-  int64_t bytes = da::state_bytes(da::plan(T, n_seq, packed != 0, H, passes), T, H, dk, dv, passes);
+  int64_t bytes = da::state_bytes(da::plan(T, n_seq, packed != 0, H, passes, da::use_tc(dtype, dk, dv)), T, H, dk, dv, passes);
   if (backward && H != Hk) bytes += 2 * (packed ? 1 : n_seq) * T * H * dk * 4;
   return bytes;
 }
@@ -315,7 +322,8 @@ extern "C" int64_t ttc_decay_attn_workspace(int64_t T, int n_seq, int packed, in
 extern "C" int ttc_decay_attn_fwd(const void* q, const void* k, const void* v, const int64_t* strides,
                                   const float* log_gamma, float scale, const float* initial_state,
                                   const int* cu_seqlens, int64_t T, int n_seq, int H, int Hk, int dk, int dv, int dtype,
-                                  void* o, float* final_state, void* workspace, int64_t workspace_bytes, void* stream) {
+                                  void* o, float* final_state, void* workspace, int64_t workspace_bytes, int* status,
+                                  void* stream) {
   if (int rc = da::check(T, n_seq, H, Hk, dk, dv, dtype)) return rc;
   if (n_seq == 0) return cu_seqlens ? da::fail(TTC_ERR_INVALID, "decay_attn: packed rows need a sequence") : TTC_OK;
   if (!strides || !log_gamma || (T > 0 && (!q || !k || !v || !o)))
@@ -323,7 +331,7 @@ extern "C" int ttc_decay_attn_fwd(const void* q, const void* k, const void* v, c
   const void* ops[3] = {q, k, v};
   for (int i = 0; i < 3; ++i)
     if (int rc = da::check_operand(ops[i], strides + 3 * i, 3, dtype)) return rc;
-  const da::Plan p = da::plan(T, n_seq, cu_seqlens != nullptr, H, 1);
+  const da::Plan p = da::plan(T, n_seq, cu_seqlens != nullptr, H, 1, da::use_tc(dtype, dk, dv));
   const int64_t need = da::state_bytes(p, T, H, dk, dv, 1);
   if (workspace_bytes < need || (need > 0 && (!workspace || da::misaligned16(workspace))))
     return da::fail(TTC_ERR_INVALID, "decay_attn_fwd: workspace missing, misaligned or smaller than ttc_decay_attn_workspace");
@@ -348,14 +356,15 @@ extern "C" int ttc_decay_attn_fwd(const void* q, const void* k, const void* v, c
   f.seg = da::segmented(p, T) ? static_cast<float*>(workspace) : nullptr;
   f.kd = dk, f.vd = dv;
   f.a = f.b = scale, f.u = 1.f;
-  return da::run_passes(A, &f, 1, dtype, f.seg != nullptr, static_cast<cudaStream_t>(stream));
+  return da::run_passes(A, &f, 1, dtype, f.seg != nullptr, da::use_tc(dtype, dk, dv), status,
+                        static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int ttc_decay_attn_bwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* g_o,
                                   const float* log_gamma, float scale, const float* initial_state,
                                   const float* g_final_state, const int* cu_seqlens, int64_t T, int n_seq, int H, int Hk,
                                   int dk, int dv, int dtype, void* d_q, void* d_k, void* d_v, float* d_initial_state,
-                                  void* workspace, int64_t workspace_bytes, void* stream) {
+                                  void* workspace, int64_t workspace_bytes, int* status, void* stream) {
   if (int rc = da::check(T, n_seq, H, Hk, dk, dv, dtype)) return rc;
   if (n_seq == 0) return cu_seqlens ? da::fail(TTC_ERR_INVALID, "decay_attn: packed rows need a sequence") : TTC_OK;
   if (!strides || !log_gamma || (T > 0 && (!q || !k || !v || !g_o || !d_q || !d_k || !d_v)))
@@ -365,7 +374,7 @@ extern "C" int ttc_decay_attn_bwd(const void* q, const void* k, const void* v, c
     if (int rc = da::check_operand(ops[i], strides + 3 * i, 3, dtype)) return rc;
   const int64_t gs[3] = {T * H * dv, static_cast<int64_t>(H) * dv, dv};
   if (int rc = da::check_operand(g_o, gs, 0, dtype)) return rc;
-  const da::Plan p = da::plan(T, n_seq, cu_seqlens != nullptr, H, 3);
+  const da::Plan p = da::plan(T, n_seq, cu_seqlens != nullptr, H, 3, da::use_tc(dtype, dk, dv));
   const int64_t sbytes = da::state_bytes(p, T, H, dk, dv, 3);
   const int grp = H / Hk;
   const int64_t rows = (cu_seqlens ? 1 : n_seq) * T;
@@ -417,7 +426,7 @@ extern "C" int ttc_decay_attn_bwd(const void* q, const void* k, const void* v, c
   dkp.init = g_final_state, dkp.isk = 1, dkp.isv = dv;
   dkp.kd = dv, dkp.vd = dk, dkp.b = 1.f, dkp.u = scale, dkp.e = 1, dkp.reverse = 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int rc = da::run_passes(A, ps, 3, dtype, ps[0].seg != nullptr, st)) return rc;
+  if (int rc = da::run_passes(A, ps, 3, dtype, ps[0].seg != nullptr, da::use_tc(dtype, dk, dv), status, st)) return rc;
   if (grp == 1 || rows == 0) return TTC_OK;
   const int64_t n4 = rows * Hk * dk / 4;
   const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((n4 + 255) / 256, 148 * 16));

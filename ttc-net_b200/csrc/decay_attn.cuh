@@ -221,6 +221,21 @@ __device__ __noinline__ void slow_pv(float (&acc)[4][4], const char* Ps, const c
     }
 }
 
+// Zeros in the rows behind the last packed sequence.
+template <bool BF16>
+__device__ __forceinline__ void zero_rows_behind(const Args& A, const Pass& P, int h, int tid, int threads) {
+  int64_t row0, len;
+  seq_range(A, A.n_seq - 1, row0, len);
+  for (int64_t r = row0 + len; r < A.T; ++r)
+    for (int c = tid; c < P.vd; c += threads) {
+      const int64_t at = (r * A.H + h) * P.vd + c;
+      if (BF16 && !P.o_f32)
+        static_cast<__nv_bfloat16*>(P.o)[at] = __float2bfloat16_rn(0.f);
+      else
+        static_cast<float*>(P.o)[at] = 0.f;
+    }
+}
+
 // STATE_ONLY: the sums u gamma^.. k^T v of the segments alone, from a zero state.
 template <int DK, int DV, int NP, bool STATE_ONLY>
 __global__ void __launch_bounds__(Shape<DK, DV, NP, STATE_ONLY>::THREADS) decay_attn_kernel(const __grid_constant__ Args A) {
@@ -234,17 +249,7 @@ __global__ void __launch_bounds__(Shape<DK, DV, NP, STATE_ONLY>::THREADS) decay_
   float* const pw = reinterpret_cast<float*>(Ps + S::PB);
 
   if (!STATE_ONLY && A.cu != nullptr && static_cast<int>(blockIdx.x) == A.items) {
-    // rows behind the last sequence: zeros
-    int64_t row0, len;
-    seq_range(A, A.n_seq - 1, row0, len);
-    for (int64_t r = row0 + len; r < A.T; ++r)
-      for (int c = tid; c < P.vd; c += S::THREADS) {
-        const int64_t at = (r * A.H + h) * P.vd + c;
-        if (NP == 1 && !P.o_f32)
-          static_cast<__nv_bfloat16*>(P.o)[at] = __float2bfloat16_rn(0.f);
-        else
-          static_cast<float*>(P.o)[at] = 0.f;
-      }
+    zero_rows_behind<NP == 1>(A, P, h, tid, S::THREADS);
     return;
   }
   const Item it = find_item(A, blockIdx.x);

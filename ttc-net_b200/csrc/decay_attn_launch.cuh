@@ -52,7 +52,8 @@ int launch(const Args& A, int passes, bool state_only, cudaStream_t st) {
   return set_error(TTC_ERR_UNSUPPORTED, "decay_attn: no kernel for these head dims");
 }
 
-int launch_bf16(const Args& A, int passes, bool state_only, cudaStream_t st);
+// bf16: `tc` picks the tcgen05 kernel (decay_attn_tc.cuh), else the warp-level one.
+int launch_bf16(const Args& A, int passes, bool state_only, bool tc, int* status, cudaStream_t st);
 int launch_f32(const Args& A, int passes, bool state_only, cudaStream_t st);
 
 }  // namespace da

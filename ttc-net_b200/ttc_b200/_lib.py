@@ -68,9 +68,9 @@ SIGNATURES = {
     "ttc_prologue_fwd": (_I, [_P, _I64] + [_I] * 6 + [_P] * 9 + [_P, _P]),
     "ttc_prologue_bwd": (_I, [_P, _I64] + [_I] * 6 + [_P] * 9 + [_P, _P]),
     "ttc_decay_attn_workspace": (_I64, [_I64] + [_I] * 8),
-    "ttc_decay_attn_fwd": (_I, [_P] * 3 + [_SP, _FP, _F, _FP, _P, _I64] + [_I] * 6 + [_P, _FP, _P, _I64, _P]),
+    "ttc_decay_attn_fwd": (_I, [_P] * 3 + [_SP, _FP, _F, _FP, _P, _I64] + [_I] * 6 + [_P, _FP, _P, _I64, _P, _P]),
     "ttc_decay_attn_bwd": (_I, [_P] * 3 + [_SP, _P, _FP, _F, _FP, _FP, _P, _I64] + [_I] * 6
-                           + [_P] * 3 + [_FP, _P, _I64, _P]),
+                           + [_P] * 3 + [_FP, _P, _I64, _P, _P]),
     "ttc_decay_attn_step": (_I, [_P] * 3 + [_SP, _FP, _F, _FP, _I64, _P] + [_I] * 7 + [_P, _P]),
     "ttc_rotary": (_I, [_P, _SP, _I, _P, _SP, _I, _P, _SP, _I, _P, _I64, _I64] + [_I] * 4 + [_F, _I] + [_P] * 3),
     "ttc_group_norm_workspace": (_I64, [_I64, _I, _I, _I]),

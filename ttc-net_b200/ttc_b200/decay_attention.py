@@ -26,6 +26,26 @@ def _workspace(nbytes: int, dev) -> torch.Tensor | None:
     return torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
 
 
+# One word of pinned host memory that every kernel can reach: it is read at the next call without
+# waiting for the GPU.
+_status: torch.Tensor | None = None
+
+WAIT_TIMEOUT_MSG = ("ttc_b200 decay_attention: a wait inside an earlier call's kernel ran out "
+                    "(that call's results are not valid)")
+
+
+def _status_word() -> int:
+    """The address of the status word; raises if a call since the last one reported a timeout."""
+    global _status
+    if _status is None:
+        _status = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+    word = ctypes.c_int.from_address(_status.data_ptr())
+    if word.value:
+        word.value = 0
+        raise RuntimeError(WAIT_TIMEOUT_MSG)
+    return _status.data_ptr()
+
+
 def _operand(t: torch.Tensor) -> torch.Tensor:
     """t itself if its head dim is contiguous and its rows start on 16-byte boundaries (a slice of
     a fused projection, an expanded tensor), else a contiguous copy."""
@@ -90,7 +110,7 @@ class DecayAttentionFunction(torch.autograd.Function):
             ws = _workspace(nbytes, dev)
             _launch("ttc_decay_attn_fwd", dev, lib.ttc_decay_attn_fwd, _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v),
                     _ptr(log_gamma), scale, _ptr(initial_state), _ptr(cu_seqlens), *dims, _ptr(o), _ptr(state),
-                    _ptr(ws), nbytes)
+                    _ptr(ws), nbytes, _status_word())
         ctx.save_for_backward(q, k, v, log_gamma, initial_state, cu_seqlens)
         ctx.dims, ctx.scale = dims, scale
         return o, state
@@ -115,7 +135,7 @@ class DecayAttentionFunction(torch.autograd.Function):
             ws = _workspace(nbytes, dev)
             _launch("ttc_decay_attn_bwd", dev, lib.ttc_decay_attn_bwd, _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v),
                     _ptr(g_o), _ptr(log_gamma), ctx.scale, _ptr(initial_state), _ptr(g_state), _ptr(cu_seqlens),
-                    *ctx.dims, _ptr(d_q), _ptr(d_k), _ptr(d_v), _ptr(d_s), _ptr(ws), nbytes)
+                    *ctx.dims, _ptr(d_q), _ptr(d_k), _ptr(d_v), _ptr(d_s), _ptr(ws), nbytes, _status_word())
         return d_q, d_k, d_v, None, None, d_s, None, None
 
 
