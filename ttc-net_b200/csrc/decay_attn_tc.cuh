@@ -1,7 +1,7 @@
 // The recurrence of decay_attn.cuh for bf16 on the 5th-generation tensor cores: one persistent-state CTA for
 // each segment of a (sequence, head), blocks of 64 tokens, five warpgroups with roles of their own.
 //
-// Products of a block (M = 128 TMEM lanes; dv or 64 tokens of them used, rows are independent):
+// Products of a block (M = 128 TMEM lanes, dv of them used, rows are independent; M = 64 for the scores):
 //   Sc [i x j]   = q k^T                A = q, B = k                  (shared memory, K-major)
 //   U  [dv x dk] = (f v)^T k            A = f v in bf16 parts, B = k  (shared memory, MN-major)
 //   O1 [dv x i]  = bf16(S)^T q^T        A = S^T in TMEM, B = q        (K-major)
@@ -12,14 +12,20 @@
 // Roles:
 //   warps 0-3    the state: row dv of S^T in DK fp32 registers of its thread, S = gamma^rows S + U
 //                with an ordinary fma (U is summed from zero in TMEM), and S in bf16 to TMEM
-//   warps 4-7    o = f_i O1 + O2, rounded and staged through the block's v tile to 16-byte stores
-//   warps 8, 9   P = scores times decays, masked, in bf16 to shared memory
-//   warp 10      issues every tcgen05.mma
+//   warps 4-7    o = f_i O1 + O2, rounded, transposed through shared memory to 16-byte stores
+//   warps 8-11   P = scores times decays, masked, in bf16 to shared memory
 //   warps 12-15  f v in two or three bf16 parts; notes blocks whose v holds Inf or NaN
-//   warps 16-18  16-byte asynchronous copies of every third block each (three stages)
-// Every wait is bounded (about two seconds); one that runs out makes all roles leave and sets
+//   warps 16-18  copies of every third block each (three stages): whole blocks by TMA, a sequence's
+//                partial last block by 16-byte asynchronous copies that write zeros for what is not in it
+//   warp 19      issues every tcgen05.mma
+// Rows of a block lie in token order; in a backward pass the later row is the earlier place.
+// Every wait is bounded (wait_bar); one that runs out makes all roles leave and sets
 // TTC_STATUS_MMA_TIMEOUT in the status word.
 #pragma once
+
+#include <cuda.h>
+
+#include <type_traits>
 
 #include "decay_attn.cuh"
 #include "tc_primitives.cuh"
@@ -37,8 +43,8 @@ struct TcShape {
   static constexpr int PB = C * C * 2;
   static constexpr int PARTS = kTcStages * STAGE;  // f v, part by part
   __host__ __device__ static constexpr int p_off(int parts) { return PARTS + parts * VB; }
-  __host__ __device__ static constexpr int tail_off(int parts) { return p_off(parts) + 2 * PB; }
-  static constexpr int smem(int parts) { return 1024 + tail_off(parts) + 1024; }
+  __host__ __device__ static constexpr int o_off(int parts) { return p_off(parts) + 2 * PB; }
+  static constexpr int smem(int parts) { return 1024 + o_off(parts) + VB; }
   // TMEM columns
   static constexpr int U = 0, S = 128, SC = 192, O = 256;  // O: two buffers of (O1 64, O2 64)
 };
@@ -48,52 +54,178 @@ struct TcBars {
       u_empty, s_full, s_empty, o_full[2], o_empty[2];
 };
 
-// Instruction descriptor: D fp32, A and B bf16, M = 128; *_mn: that operand is MN-major.
-__host__ __device__ constexpr uint32_t idesc_bf16(int n, bool a_mn, bool b_mn) {
+// Tensor maps [batch, head, token, dim], boxes of 64 tokens x 64 dims, 128-byte swizzle: a pass reads q, k, v
+// through maps number m[pass][0 .. 2] and writes o, where that is bf16, through out[pass].
+struct TcMaps {
+  CUtensorMap map[4], out[3];
+  int m[3][3];
+};
+
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int row, int head, int batch,
+                                        uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(row), "r"(head), "r"(batch), "r"(tc::smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc::smem_u32(bar)), "r"(bytes) : "memory");
+}
+
+// Instruction descriptor: D fp32, A and B bf16; *_mn: that operand is MN-major.
+__host__ __device__ constexpr uint32_t idesc_bf16(int m, int n, bool a_mn, bool b_mn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
-         (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
-// Shared-memory descriptor, 128-byte swizzle: 8-row groups 1024 bytes apart, 64-column halves 8192.
-__device__ __forceinline__ uint64_t desc128(uint32_t addr) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3fffu) | (static_cast<uint64_t>(8192 >> 4) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Shared-memory descriptor, 128-byte swizzle, 8-row groups 1024 bytes apart, 64-column halves 8192: the
+// upper word is a constant, the lower one moves by bytes / 16.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr) { return (addr >> 4) | ((8192u >> 4) << 16); }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, q;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 q, %4, 0;\n\t"
+      "mov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, q;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kDescHi)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, q;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred q;\n\t.reg .b64 y;\n\tsetp.ne.b32 q, %4, 0;\n\tmov.b64 y, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, q;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kDescHi)
       : "memory");
+}
+// 16 lanes x 64 columns in the layout of mma accumulators: v[4 n + x] is lane g + 8 (x >> 1), column
+// 8 n + 2 t + (x & 1) of thread (g, t) = (lane / 4, lane % 4).  No wait.
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+        "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+        "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_wait_ld(float (&a)[32], float (&b)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  // the loaded registers are not to be read before the wait
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(a[i]), "+f"(b[i]));
+}
+// The same for 16 columns.
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, float (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(float (&a)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) asm volatile("" : "+f"(a[i]));
+}
+// Four 8x8 matrices of 16-bit values.
+__device__ __forceinline__ void stsm4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+               "r"(d)
+               : "memory");
+}
+// The same, each stored transposed.
+__device__ __forceinline__ void stsm4t(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b),
+               "r"(c), "r"(d)
+               : "memory");
+}
+// (a, b) = (x, y) (a, b) + (c, d), rounded as two fmas.
+__device__ __forceinline__ void fma2(float& a, float& b, float x, float y, float c, float d) {
+  asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmov.b64 r, {%4, %5};\n\t"
+      "fma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(x), "f"(y), "f"(c), "f"(d));
+}
+__device__ __forceinline__ void tma_out(const CUtensorMap* map, uint32_t src, int x, int row, int head, int batch) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map), "r"(src),
+               "r"(x), "r"(row), "r"(head), "r"(batch)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// PARTS bf16 parts of f times the two bf16 values in u (no care for Inf: such blocks are noted anyway).
+template <int PARTS>
+__device__ __forceinline__ void decayed(uint32_t u, float f, uint32_t (&o)[PARTS]) {
+  float x, y;
+  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %4};\n\tmul.rn.f32x2 p, p, q;\n\t"
+      "mov.b64 {%0, %1}, p;\n\t}"
+      : "=f"(x), "=f"(y)
+      : "f"(mma::lo_f(u)), "f"(mma::hi_f(u)), "f"(f));
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    o[p] = mma::pack2(x, y);
+    if (p + 1 < PARTS)
+      asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tsub.rn.f32x2 p, p, q;\n\t"
+          "mov.b64 {%0, %1}, p;\n\t}"
+          : "+f"(x), "+f"(y)
+          : "f"(mma::lo_f(o[p])), "f"(mma::hi_f(o[p])));
+  }
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(bar)) : "memory");
 }
 
-// Phase `parity` of `bar`, for a whole warp: false for all lanes once the time is up or another role has given up.
+__device__ __forceinline__ uint32_t bar_try(uint32_t addr, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(addr), "r"(parity)
+      : "memory");
+  return done;
+}
+// Phase `parity` of `bar`, for a whole warp: false for all lanes after two million polls (each sleeps up to a
+// microsecond) or once another role has given up.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* gone) {
   const uint32_t addr = tc::smem_u32(bar);
-  uint64_t t0 = 0;
-  for (;;) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 10000;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(addr), "r"(parity)
-        : "memory");
-    if (__all_sync(0xffffffffu, done)) return true;
-    const uint64_t t = tc::global_ns();
-    if (t0 == 0) t0 = t;
-    if (t - t0 > 2000000000ull) *gone = 1;
+#pragma unroll 1
+  for (int n = 0; n < 2000000; ++n) {
+    if (__all_sync(0xffffffffu, bar_try(addr, parity))) return true;
     if (__any_sync(0xffffffffu, *gone != 0)) return false;
   }
+  *gone = 1;
+  return false;
+}
+
+// The same without waiting.
+__device__ __forceinline__ bool bar_done(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(tc::smem_u32(bar)), "r"(parity)
+      : "memory");
+  return __all_sync(0xffffffffu, done);
+}
+
+// Named barrier that tells every thread whether all of them had `ok`.
+__device__ __forceinline__ bool sync_all(int id, int count, bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(static_cast<uint32_t>(ok)), "r"(id), "r"(count)
+      : "memory");
+  return all != 0;
 }
 
 template <int N>
@@ -111,8 +243,38 @@ __device__ __forceinline__ float bf_at(const char* tile, int r, int col) {
       *reinterpret_cast<const __nv_bfloat16*>(tile + (col >> 6) * 8192 + swz(r, (col & 63) >> 3) + (col & 7) * 2));
 }
 
+__device__ __forceinline__ float tmem_ld_one(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;" : "=r"(r) : "r"(taddr) : "memory");
+  return __uint_as_float(r);
+}
+
+// The outputs of a warp's 32 value rows where v holds Inf or NaN, whose products with masked zeros are NaN: the
+// scores' product term by term over the past tokens only.  Lane l: value row v0 + l.
+__device__ __noinline__ void outputs_by_term(const Pass& P, uint32_t o1, const char* pt, const char* vt, const float* pw,
+                                             int v0, int lo, int hi, int64_t at, int64_t row) {
+  const int vr = v0 + (threadIdx.x & 31);
+#pragma unroll 1
+  for (int i = 0; i < C; ++i) {
+    __syncwarp();
+    const float o = tmem_ld_one(o1 + i);
+    if (vr < P.vd && i >= lo && i < hi) {
+      float a = 0.f;
+#pragma unroll 1
+      for (int j = P.reverse ? i : 0; j <= (P.reverse ? C - 1 : i); ++j) a = fmaf(bf_at(pt, i, j), bf_at(vt, j, vr), a);
+      a = fmaf(P.b * pw[(P.reverse ? C - 1 - i : i) + 1 - P.e], o, a);
+      const int64_t e = at + i * row + vr;
+      if (P.o_f32)
+        static_cast<float*>(P.o)[e] = a;
+      else
+        static_cast<__nv_bfloat16*>(P.o)[e] = __float2bfloat16_rn(a);
+    }
+  }
+  __syncwarp();
+}
+
 template <int DK, int DV, bool STATE_ONLY>
-__global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __grid_constant__ Args A, int* status) {
+__global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __grid_constant__ Args A, const __grid_constant__ TcMaps M, int* status) {
   using S = TcShape<DK, DV>;
   extern __shared__ char smem_raw[];
   __shared__ TcBars bars;
@@ -122,7 +284,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
   char* const smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
   const Pass& P = A.pass[blockIdx.z];
   const int h = blockIdx.y;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
   if (!STATE_ONLY && A.cu != nullptr && static_cast<int>(blockIdx.x) == A.items) {
     zero_rows_behind<true>(A, P, h, tid, kTcThreads);
@@ -138,6 +300,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
   const bool keep_last = STATE_ONLY || (P.seg == nullptr && P.fin != nullptr);  // the state behind the last block
   const int parts = A.parts;
 
+  const bool rev = P.reverse != 0;
+  const int bi = A.cu == nullptr ? it.seq : 0;
+  // row of the first block's first row in token order; blocks follow 64 rows up or down
+  const int64_t first = rev ? it.row0 + it.len - s0 - C : it.row0 + s0;
+  const int64_t down = rev ? -C : C;
+
   volatile int* const gone = &gone_s;
   if (tid == 0) {
     for (int i = 0; i < kTcStages; ++i) {
@@ -146,7 +314,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
       bad_s[i] = 0;
     }
     tc::mbar_init(&bars.sc_full, 1);
-    tc::mbar_init(&bars.sc_empty, 2);
+    tc::mbar_init(&bars.sc_empty, 4);
     tc::mbar_init(&bars.vs_full, 4);
     tc::mbar_init(&bars.vs_empty, 1);
     tc::mbar_init(&bars.u_full, 1);
@@ -154,7 +322,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
     tc::mbar_init(&bars.s_full, 4);
     tc::mbar_init(&bars.s_empty, 1);
     for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&bars.p_full[i], 2);
+      tc::mbar_init(&bars.p_full[i], 4);
       tc::mbar_init(&bars.p_empty[i], 4);
       tc::mbar_init(&bars.o_full[i], 1);
       tc::mbar_init(&bars.o_empty[i], 4);
@@ -163,7 +331,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
     tc::mbar_init_fence();
   }
   if (tid >= 64 && tid <= 64 + C) pw[tid - 64] = decay_pow(A.log_gamma[h], tid - 64);
-  if (warp == 11) tc::tmem_alloc(&tmem_base, 512);
+  if (warp == 19) tc::tmem_alloc(&tmem_base, 512);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -189,6 +357,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
     float st[DK];
 #pragma unroll
     for (int k = 0; k < DK; ++k) st[k] = src != nullptr && k < P.kd && vr < P.vd ? src[k * sk + vr * sv] : 0.f;
+#pragma unroll 1
     for (int c = 0; c < blocks; ++c) {
       const int rows = min(C, seg_rows - c * C);
       if (!STATE_ONLY) {
@@ -215,7 +384,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
           float u[32];
           tc::tmem_ld<32>(my + S::U + 32 * x, u);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) st[32 * x + i] = fmaf(keep, st[32 * x + i], u[i]);
+          for (int i = 0; i < 32; i += 2) fma2(st[32 * x + i], st[32 * x + i + 1], keep, keep, u[i], u[i + 1]);
         }
         tc::fence_before_sync();
         __syncwarp();
@@ -237,137 +406,269 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
     }
   } else if (warp < 8) {  // ------------------------------------------------------------ the outputs
     if (!STATE_ONLY) {
-      const int w4 = warp - 4, vr = w4 * 32 + lane, t4 = tid - 128;
-      const uint32_t my = tm + (static_cast<uint32_t>(w4 * 32) << 16);
-      const int bi = A.cu == nullptr ? it.seq : 0;
-      const int64_t step = P.reverse ? -1 : 1;
-      const int64_t tok0 = bi * A.T + it.row0 + (P.reverse ? it.len - 1 - s0 : s0);
-      const bool live = w4 * 32 < P.vd;
-      for (int c = 0; c < blocks; ++c) {
-        const int rows = min(C, seg_rows - c * C), s = c % kTcStages, b = c & 1;
-        if (!wait_bar(&bars.o_full[b], (c >> 1) & 1, gone)) break;
-        tc::fence_after_sync();
-        char* const vt = smem + s * S::STAGE + 2 * S::KB;
-        const bool bad = *static_cast<volatile int*>(&bad_s[s]) == c + 1;
-        uint32_t out[2][16];
-        float* const of = static_cast<float*>(P.o);
-        const char* const pt = smem + S::p_off(parts) + b * S::PB;
+      const int w4 = warp - 4, g = lane >> 2, t = lane & 3, m = lane >> 3, r8 = lane & 7, v0 = w4 * 32;
+      const uint32_t my = tm + (static_cast<uint32_t>(w4 * 32) << 16) + S::O;
+      const uint32_t ot = tc::smem_u32(smem) + S::o_off(parts);
+      const int64_t row = static_cast<int64_t>(A.H) * P.vd;  // elements between a head's tokens
+      int64_t at = (bi * A.T + first) * row + h * static_cast<int64_t>(P.vd);  // the block's first row
+      float f[8][2];  // of rows 8 n + 2 t (+ 1)
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          float o1[32], o2[32];
-          tc::tmem_ld<32>(my + S::O + 128 * b + 32 * x, o1);
-          tc::tmem_ld<32>(my + S::O + 128 * b + 64 + 32 * x, o2);
-          if (bad) {  // 0 * NaN: term by term over j <= i
+          const int i = 8 * n + 2 * t + x;
+          f[n][x] = P.b * pw[(rev ? C - 1 - i : i) + 1 - P.e];
+        }
 #pragma unroll 1
-            for (int i = 0; i < 32; ++i) {
-              float a = 0.f;
-              for (int j = 0; j <= 32 * x + i; ++j)
-                if (vr < P.vd) a = fmaf(bf_at(pt, 32 * x + i, j), bf_at(vt, j, vr), a);
-              // registers are indexed by constants only
+      for (int c = 0; c < blocks; ++c, at += down * row) {
+        const int rows = min(C, seg_rows - c * C), s = c % kTcStages, b = c & 1;
+        const int lo = rev ? C - rows : 0, hi = lo + rows;  // the block's rows that are in the sequence
+        bool ok = wait_bar(&bars.o_full[b], (c >> 1) & 1, gone);
+        if (tid == 128) bulk_wait_read();  // the staging has left
+        // all four warps go on or none
+        if (!sync_all(1, 128, ok)) break;
+        tc::fence_after_sync();
+        const bool bad = *static_cast<volatile int*>(&bad_s[s]) == c + 1;
+        if (bad)
+          outputs_by_term(P, my + 128 * b, smem + S::p_off(parts) + b * S::PB, smem + s * S::STAGE + 2 * S::KB, pw, v0, lo,
+                          hi, at, row);
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bars.p_empty[b]);
+          mbar_arrive(&bars.empty[s]);
+        }
+        if (!bad) {
+#pragma unroll 1
+          for (int hl = 0; hl < 2; ++hl) {
+            const int vh = v0 + 16 * hl;
+            if (vh < P.vd) {
+              float o1[32], o2[32];
+              tmem_ld_frag(my + (16u << 16) * hl + 128 * b, o1);
+              tmem_ld_frag(my + (16u << 16) * hl + 128 * b + 64, o2);
+              tmem_wait_ld(o1, o2);
 #pragma unroll
-              for (int q = 0; q < 32; ++q)
-                if (q == i) o2[q] = a;
+              for (int q = 0; q < 32; q += 2) fma2(o1[q], o1[q + 1], f[q >> 2][0], f[q >> 2][1], o2[q], o2[q + 1]);
+              if (!P.o_f32) {
+#pragma unroll
+                for (int n = 0; n < 8; n += 2)
+                  stsm4t(ot + (vh >> 6) * 8192 + swz(8 * (n + (m >> 1)) + r8, ((vh & 63) >> 3) + (m & 1)),
+                         mma::pack2(o1[4 * n], o1[4 * n + 1]), mma::pack2(o1[4 * n + 2], o1[4 * n + 3]),
+                         mma::pack2(o1[4 * n + 4], o1[4 * n + 5]), mma::pack2(o1[4 * n + 6], o1[4 * n + 7]));
+              } else {
+                float* const of = static_cast<float*>(P.o) + at + vh + g;
+                const bool v8 = vh + g + 8 < P.vd;  // widths are multiples of 8: row g is there
+#pragma unroll
+                for (int q = 0; q < 32; ++q) {
+                  const int i = 8 * (q >> 2) + 2 * t + (q & 1);
+                  if (i >= lo && i < hi && (!(q & 2) || v8)) of[i * row + 4 * (q & 2)] = o1[q];
+                }
+              }
             }
-          }
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o1[i] = fmaf(P.b * pw[32 * x + i + 1 - P.e], o1[i], o2[i]);
-          if (P.o_f32) {
-            if (vr < P.vd) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (32 * x + i < rows)
-                  of[((tok0 + step * (c * C + 32 * x + i)) * A.H + h) * P.vd + vr] = o1[i];
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) out[x][i] = mma::pack2(o1[2 * i], o1[2 * i + 1]);
           }
         }
         tc::fence_before_sync();
-        if (bad) tc::named_sync(1, 128);  // all of v is read before it is overwritten
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bars.o_empty[b]);
-          mbar_arrive(&bars.p_empty[b]);
-        }
-        if (!P.o_f32) {
-          // rows of DV values; the last readers of the v tile are done (this block's O2)
-          if (live) {
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                char* p = vt + (32 * x + 2 * i) * (DV * 2) + vr * 2;
-                *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(out[x][i]);
-                *reinterpret_cast<uint16_t*>(p + DV * 2) = static_cast<uint16_t>(out[x][i] >> 16);
-              }
-          }
+        if (lane == 0) mbar_arrive(&bars.o_empty[b]);
+        if (!P.o_f32 && !bad) {
+          tc::fence_smem_to_async();
           tc::named_sync(1, 128);
-          __nv_bfloat16* const ob = static_cast<__nv_bfloat16*>(P.o);
-          for (int x = t4; x < C * (DV / 8); x += 128) {
-            const int i = x / (DV / 8), p8 = x % (DV / 8);
-            if (i < rows && p8 * 8 < P.vd)
-              *reinterpret_cast<uint4*>(ob + ((tok0 + step * (c * C + i)) * A.H + h) * P.vd + p8 * 8) =
-                  *reinterpret_cast<const uint4*>(vt + i * (DV * 2) + p8 * 16);
+          if (rows == C) {
+            if (tid == 128) {
+#pragma unroll
+              for (int hf = 0; hf < DV / 64; ++hf)
+                if (hf * 64 < P.vd)
+                  tma_out(&M.out[blockIdx.z], ot + hf * 8192, hf * 64, static_cast<int>(first + down * c), h, bi);
+              bulk_commit();
+            }
+          } else {  // the rows beyond are not this sequence's
+#pragma unroll 1
+            for (int x = tid - 128; x < C * DV / 8; x += 128) {
+              const int i = x / (DV / 8), p8 = x % (DV / 8);
+              if (i >= lo && i < hi && p8 * 8 < P.vd)
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(P.o) + at + i * row + p8 * 8) =
+                    *reinterpret_cast<const uint4*>(smem + S::o_off(parts) + (p8 >> 3) * 8192 + swz(i, p8 & 7));
+            }
           }
         }
+      }
+      if (tid == 128) bulk_wait();
+    }
+  } else if (warp < 12) {  // ---------------------------------------------------------------- the scores
+    regs_dec<72>();
+    if (!STATE_ONLY) {
+      // Warp w has rows 16 w .. 16 w + 15 (M = 64: TMEM lanes 32 w ..), a thread rows g and g + 8, columns
+      // 8 n + 2 t + x.  The decay of |i - j| places on the past side (j <= i, or j >= i backwards) is
+      // gamma^(whole groups of 8 between them) times a constant of the thread with 1 to 14 places; in the group that
+      // holds the diagonal it is `own`, 0 beyond it.  No negative powers, whatever gamma.
+      const int w = warp - 8, g = lane >> 2, t = lane & 3, m = lane >> 3, r8 = lane & 7;
+      const uint32_t my = tm + (static_cast<uint32_t>(w * 32) << 16) + S::SC;
+      float edge[2], own[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int d = rev ? 2 * t + x - g : g - 2 * t - x;
+        edge[x] = pw[8 + d];
+        own[x] = d >= 0 ? P.a * pw[max(d, 0)] : 0.f;
+      }
+      bool see[2] = {rev ? 2 * t >= g : g >= 2 * t, rev ? 2 * t + 1 >= g : g >= 2 * t + 1};
+#pragma unroll 1
+      for (int c = 0; c < blocks; ++c) {
+        const int b = c & 1;
+        if (c > 1 && !wait_bar(&bars.p_empty[b], ((c >> 1) - 1) & 1, gone)) break;
+        if (!wait_bar(&bars.sc_full, c & 1, gone)) break;
+        tc::fence_after_sync();
+        const uint32_t pt = tc::smem_u32(smem) + S::p_off(parts) + b * S::PB;
+        float v[8], next[8];
+        tmem_ld_frag(my, next);
+#pragma unroll 1
+        for (int n = 0; n < 8; n += 2) {
+          tmem_wait_ld(next);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) v[x] = next[x];
+          if (n < 6) {
+            tmem_ld_frag(my + 8 * n + 16, next);
+          } else {
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.sc_empty);
+          }
+          uint32_t o[2][2];
+#pragma unroll
+          for (int z = 0; z < 2; ++z)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {  // columns of group n + z, rows g + 8 y: group number 2 w + y
+              const int away = rev ? n + z - 2 * w - y : 2 * w + y - n - z;  // the same for the whole warp
+              float a = v[4 * z + 2 * y], d = v[4 * z + 2 * y + 1];
+              if (away > 0) {
+                const float f = P.a * pw[8 * away - 8];
+                a *= f * edge[0];
+                d *= f * edge[1];
+              } else {  // selects, not products with 0: masked scores may be Inf or NaN
+                a = away == 0 && see[0] ? a * own[0] : 0.f;
+                d = away == 0 && see[1] ? d * own[1] : 0.f;
+              }
+              o[z][y] = mma::pack2(a, d);
+            }
+          // matrices (rows 8 y, columns 8 n)
+          stsm4(pt + swz(16 * w + 8 * (m & 1) + r8, n + (m >> 1)), o[0][0], o[0][1], o[1][0], o[1][1]);
+        }
+        tc::fence_smem_to_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.empty[s]);
+        if (lane == 0) mbar_arrive(&bars.p_full[b]);
       }
     }
-  } else if (warp < 12) {
+  } else if (warp < 16) {  // ----------------------------------------------------- the decayed values
     regs_dec<64>();
-    if (warp < 10) {  // ---------------------------------------------------------------- the scores
-      if (!STATE_ONLY) {
-        const int i = (warp - 8) * 32 + lane;
-        const uint32_t my = tm + (static_cast<uint32_t>((warp - 8) * 32) << 16) + S::SC;
-        for (int c = 0; c < blocks; ++c) {
-          const int b = c & 1;
-          if (c > 1 && !wait_bar(&bars.p_empty[b], ((c >> 1) - 1) & 1, gone)) break;
-          if (!wait_bar(&bars.sc_full, c & 1, gone)) break;
-          tc::fence_after_sync();
-          char* const pt = smem + S::p_off(parts) + b * S::PB;
+    const int t4 = tid - 384;
+    const uint32_t my_off = swz(t4 >> 3, t4 & 7);  // of row t4 / 8; rows 16 further have the same swizzle
+#pragma unroll 1
+    for (int c = 0; c < blocks; ++c) {
+      const int rows = min(C, seg_rows - c * C), s = c % kTcStages;
+      if (!wait_bar(&bars.full[s], (c / kTcStages) & 1, gone)) break;
+      if (c > 0 && !wait_bar(&bars.vs_empty, (c - 1) & 1, gone)) break;
+      const char* const vt = smem + s * S::STAGE + 2 * S::KB;
+      __nv_bfloat162 chk = __floats2bfloat162_rn(0.f, 0.f);
+      auto scale = [&](auto tag) {
+        constexpr int N = decltype(tag)::value;
+#pragma unroll 2
+        for (int x = 0; x < C * DV / 8 / 128; ++x) {
+          const int r = ((x * 16) & 63) + (t4 >> 3);
+          const uint32_t off = (x >> 2) * 8192 + ((x & 3) * 16) * 128 + my_off;
+          const uint4 w = *reinterpret_cast<const uint4*>(vt + off);
+          const int at = rev ? C - 1 - r : r;  // place in the block
+          const float f = at < rows ? P.u * pw[max(rows - 1 - at + P.e, 0)] : 0.f;
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+          uint32_t o[4][N];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            float v[32];
-            tc::tmem_ld<32>(my + 32 * x, v);
-            if (x == 1) {
-              tc::fence_before_sync();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&bars.sc_empty);
-            }
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              uint32_t w[4];
-#pragma unroll
-              for (int z = 0; z < 4; ++z) {
-                const int j = 32 * x + 8 * y + 2 * z, e = 8 * y + 2 * z;
-                const float v0 = j <= i ? v[e] * (P.a * pw[max(i - j, 0)]) : 0.f;
-                const float v1 = j + 1 <= i ? v[e + 1] * (P.a * pw[max(i - j - 1, 0)]) : 0.f;
-                w[z] = mma::pack2(v0, v1);
-              }
-              *reinterpret_cast<uint4*>(pt + swz(i, 4 * x + y)) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+          for (int y = 0; y < 4; ++y) {
+            chk = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&u[y]), __floats2bfloat162_rn(0.f, 0.f), chk);
+            decayed<N>(u[y], f, o[y]);
           }
+#pragma unroll
+          for (int p = 0; p < N; ++p)
+            *reinterpret_cast<uint4*>(smem + S::PARTS + p * S::VB + off) = make_uint4(o[0][p], o[1][p], o[2][p], o[3][p]);
+        }
+      };
+      if (parts == 3)
+        scale(std::integral_constant<int, 3>{});
+      else
+        scale(std::integral_constant<int, 2>{});
+      if (__low2float(chk) != 0.f || __high2float(chk) != 0.f)  // NaN too
+        *static_cast<volatile int*>(&bad_s[s]) = c + 1;
+      tc::fence_smem_to_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.vs_full);
+    }
+  } else {
+    regs_dec<56>();
+    if (warp < 16 + kTcStages) {  // ------------------------------------------------------- the copies
+      const int s = warp - 16;
+      const uint32_t base = tc::smem_u32(smem) + s * S::STAGE;
+      const CUtensorMap* const maps[3] = {&M.map[M.m[blockIdx.z][0]], &M.map[M.m[blockIdx.z][1]],
+                                          &M.map[M.m[blockIdx.z][2]]};
+      const int hq = h / P.qg, hk = h / P.kg, hv = h / P.vg;
+      // a partial block: rows lane / 8, + 4, ..; 8 lanes copy a row's 128 bytes of one half
+      auto tile = [&](uint32_t dst, const void* t, const int64_t* strides, int head, int halves, int d, int64_t row,
+                      int lo, int hi) {
+        const char* src = static_cast<const char*>(t) + (bi * strides[0] + head * strides[2]) * 2;
+        for (int hf = 0; hf < halves; ++hf)
+#pragma unroll 1
+          for (int r = lane >> 3; r < C; r += 4) {
+            const int x = hf * 64 + (lane & 7) * 8;
+            const bool on = r >= lo && r < hi && x < d;
+            mma::cp16(dst + hf * 8192 + swz(r, lane & 7), on ? src + ((row + r) * strides[1] + x) * 2 : src, on ? 16 : 0);
+          }
+      };
+      int last = -1;
+#pragma unroll 1
+      for (int c = s; c < blocks; c += kTcStages) {
+        const int rows = min(C, seg_rows - c * C);
+        if (c >= kTcStages && !wait_bar(&bars.empty[s], ((c / kTcStages) - 1) & 1, gone)) break;
+        const int64_t row = first + down * c;
+        last = c;
+        if (rows == C) {
+          if (tc::elect_one()) {
+            constexpr int BOXES = (STATE_ONLY ? 1 : 2) * (DK / 64) + DV / 64;
+            mbar_expect(&bars.full[s], BOXES * 8192);
+            const int r = static_cast<int>(row);
+#pragma unroll
+            for (int hf = 0; hf < DK / 64; ++hf) {
+              if (!STATE_ONLY) tma_box(base + hf * 8192, maps[0], hf * 64, r, hq, bi, &bars.full[s]);
+              tma_box(base + S::KB + hf * 8192, maps[1], hf * 64, r, hk, bi, &bars.full[s]);
+            }
+#pragma unroll
+            for (int hf = 0; hf < DV / 64; ++hf)
+              tma_box(base + 2 * S::KB + hf * 8192, maps[2], hf * 64, r, hv, bi, &bars.full[s]);
+          }
+          __syncwarp();
+        } else {
+          const int lo = rev ? C - rows : 0, hi = lo + rows;
+          if (!STATE_ONLY) tile(base, P.q, P.qs, hq, DK / 64, P.kd, row, lo, hi);
+          tile(base + S::KB, P.k, P.ks, hk, DK / 64, P.kd, row, lo, hi);
+          tile(base + 2 * S::KB, P.v, P.vs, hv, DV / 64, P.vd, row, lo, hi);
+          mma::cp_commit();
+          mma::cp_wait<0>();
           tc::fence_smem_to_async();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.p_full[b]);
+          if (lane == 0) mbar_arrive(&bars.full[s]);
         }
       }
-    } else if (warp == 10) {  // ------------------------------------------------------------- the MMAs
-      const uint32_t base = tc::smem_u32(smem);
+      // no copy is left in flight, whatever made the roles leave
+      if (last >= 0) tc::mbar_wait(&bars.full[s], (last / kTcStages) & 1, 0, 10000);
+    } else {  // ----------------------------------------------------------------------- the MMAs
+      const uint32_t base = desc_lo(tc::smem_u32(smem));  // descriptors count in units of 16 bytes
       const int kd16 = (P.kd + 15) / 16;
-      constexpr uint32_t d_sc = idesc_bf16(64, false, false), d_u = idesc_bf16(DK, true, true),
-                         d_o2 = idesc_bf16(64, true, false);
+      constexpr uint32_t d_sc = idesc_bf16(64, 64, false, false), d_u = idesc_bf16(128, DK, true, true),
+                         d_o1 = idesc_bf16(128, 64, false, false), d_o2 = idesc_bf16(128, 64, true, false);
       auto scores = [&](int c) {
-        const uint32_t q = base + (c % kTcStages) * S::STAGE, k = q + S::KB;
+        const uint32_t q = base + (c % kTcStages) * (S::STAGE / 16), k = q + S::KB / 16;
         if (!wait_bar(&bars.full[c % kTcStages], (c / kTcStages) & 1, gone)) return false;
         if (c > 0 && !wait_bar(&bars.sc_empty, (c - 1) & 1, gone)) return false;
         tc::fence_after_sync();
-        if (lane == 0) {
+        if (tc::elect_one()) {
+#pragma unroll 2
           for (int x = 0; x < kd16; ++x) {
-            const uint32_t off = (x >> 2) * 8192 + (x & 3) * 32;
-            mma_ss(tm + S::SC, desc128(q + off), desc128(k + off), d_sc, x > 0);
+            const uint32_t off = (x >> 2) * 512 + (x & 3) * 2;
+            mma_ss(tm + S::SC, q + off, k + off, d_sc, x > 0);
           }
           tc::mma_commit(&bars.sc_full);
         }
@@ -375,18 +676,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
         return true;
       };
       bool ok = STATE_ONLY || blocks == 0 || scores(0);
+#pragma unroll 1
       for (int c = 0; ok && c < blocks; ++c) {
         const int s = c % kTcStages, b = c & 1;
-        const uint32_t q = base + s * S::STAGE, k = q + S::KB, v = k + S::KB;
+        const uint32_t q = base + s * (S::STAGE / 16), k = q + S::KB / 16, v = k + S::KB / 16;
         if (!(ok = wait_bar(&bars.vs_full, c & 1, gone))) break;
         if (c + 1 < blocks || keep_last) {
           if (c > 0 && !(ok = wait_bar(&bars.u_empty, (c - 1) & 1, gone))) break;
           tc::fence_after_sync();
-          if (lane == 0) {
+          if (tc::elect_one()) {
+            // the small parts first
+#pragma unroll 1
             for (int p = parts - 1; p >= 0; --p)
+#pragma unroll 2
               for (int x = 0; x < C / 16; ++x)
-                mma_ss(tm + S::U, desc128(base + S::PARTS + p * S::VB + x * 2048), desc128(k + x * 2048), d_u,
-                       p < parts - 1 || x > 0);
+                mma_ss(tm + S::U, base + (S::PARTS + p * S::VB) / 16 + x * 128, k + x * 128, d_u, p < parts - 1 || x > 0);
             tc::mma_commit(&bars.vs_empty);
             tc::mma_commit(&bars.u_full);
           }
@@ -396,106 +700,34 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
         if (!(ok = wait_bar(&bars.s_full, c & 1, gone))) break;
         if (c > 1 && !(ok = wait_bar(&bars.o_empty[b], ((c >> 1) - 1) & 1, gone))) break;
         tc::fence_after_sync();
-        if (lane == 0) {
+        if (tc::elect_one()) {
+#pragma unroll 2
           for (int x = 0; x < kd16; ++x)
-            mma_ts(tm + S::O + 128 * b, tm + S::S + x * 8, desc128(q + (x >> 2) * 8192 + (x & 3) * 32), d_sc, x > 0);
+            mma_ts(tm + S::O + 128 * b, tm + S::S + x * 8, q + (x >> 2) * 512 + (x & 3) * 2, d_o1, x > 0);
           tc::mma_commit(&bars.s_empty);
         }
         __syncwarp();
-        if (c + 1 < blocks && !(ok = scores(c + 1))) break;
+        // this block's last product next if its scores are there, the next block's scores if only its data is
+        const bool early = c + 1 < blocks && !bar_done(&bars.p_full[b], (c >> 1) & 1) &&
+                           bar_done(&bars.full[(c + 1) % kTcStages], ((c + 1) / kTcStages) & 1);
+        if (early && !(ok = scores(c + 1))) break;
         if (!(ok = wait_bar(&bars.p_full[b], (c >> 1) & 1, gone))) break;
         tc::fence_after_sync();
-        if (lane == 0) {
-          const uint32_t p = base + S::p_off(parts) + b * S::PB;
-          for (int x = 0; x < C / 16; ++x)
-            mma_ss(tm + S::O + 128 * b + 64, desc128(v + x * 2048), desc128(p + x * 32), d_o2, x > 0);
+        if (tc::elect_one()) {
+          const uint32_t p = base + S::p_off(parts) / 16 + b * (S::PB / 16);
+#pragma unroll 2
+          for (int x = 0; x < C / 16; ++x) mma_ss(tm + S::O + 128 * b + 64, v + x * 128, p + x * 2, d_o2, x > 0);
           tc::mma_commit(&bars.o_full[b]);
         }
         __syncwarp();
+        if (!early && c + 1 < blocks && !(ok = scores(c + 1))) break;
       }
-    }
-  } else if (warp < 16) {  // ----------------------------------------------------- the decayed values
-    regs_dec<64>();
-    const int t4 = tid - 384;
-    for (int c = 0; c < blocks; ++c) {
-      const int rows = min(C, seg_rows - c * C), s = c % kTcStages;
-      if (!wait_bar(&bars.full[s], (c / kTcStages) & 1, gone)) break;
-      const bool update = c + 1 < blocks || keep_last;
-      if (c > 0 && !wait_bar(&bars.vs_empty, (c - 1) & 1, gone)) break;
-      const char* const vt = smem + s * S::STAGE + 2 * S::KB;
-      float chk = 0.f;
-#pragma unroll 2
-      for (int x = t4; x < C * DV / 8; x += 128) {
-        const int half = x / 512, r = (x >> 3) & 63;
-        const uint32_t off = half * 8192 + swz(r, x & 7);
-        const uint4 w = *reinterpret_cast<const uint4*>(vt + off);
-        const float f = r < rows ? P.u * pw[max(rows - 1 - r + P.e, 0)] : 0.f;
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-        uint32_t o[4][3];
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const float a = mma::lo_f(u[y]), d = mma::hi_f(u[y]);
-          chk = fmaf(a, 0.f, fmaf(d, 0.f, chk));
-          mma::split2<3>(a * f, d * f, o[y]);
-        }
-        if (update) {
-          for (int p = 0; p < 3; ++p)
-            if (p < parts)
-              *reinterpret_cast<uint4*>(smem + S::PARTS + p * S::VB + off) =
-                  make_uint4(o[0][p], o[1][p], o[2][p], o[3][p]);
-        }
-      }
-      if (chk != 0.f) *static_cast<volatile int*>(&bad_s[s]) = c + 1;  // NaN too
-      tc::fence_smem_to_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.vs_full);
-    }
-  } else {
-    regs_dec<64>();
-    if (warp < 16 + kTcStages) {  // ------------------------------------------------------- the copies
-      const int s = warp - 16;
-      const int bi = A.cu == nullptr ? it.seq : 0;
-      const char* qb = static_cast<const char*>(P.q) + (bi * P.qs[0] + (h / P.qg) * P.qs[2]) * 2;
-      const char* kb = static_cast<const char*>(P.k) + (bi * P.ks[0] + (h / P.kg) * P.ks[2]) * 2;
-      const char* vb = static_cast<const char*>(P.v) + (bi * P.vs[0] + (h / P.vg) * P.vs[2]) * 2;
-      const int64_t step = P.reverse ? -1 : 1;
-      const int64_t first = it.row0 + (P.reverse ? it.len - 1 - s0 : s0);
-      const uint32_t base = tc::smem_u32(smem) + s * S::STAGE;
-      const int piece = lane & 7, r4 = lane >> 3;
-      // rows r4, r4 + 4, ... of a tile: 8 lanes copy a row's 128 bytes of one half
-      auto tile = [&](uint32_t dst, const char* src, int64_t row_stride, int halves, int d, int64_t f, int rows) {
-        for (int hf = 0; hf < halves; ++hf) {
-          const bool col = hf * 64 + piece * 8 < d;
-          const char* p = src + ((f + step * r4) * row_stride + hf * 64 + piece * 8) * 2;
-          const int64_t next = step * row_stride * 8;
-#pragma unroll 4
-          for (int r = r4; r < C; r += 4) {
-            const bool on = col && r < rows;
-            mma::cp16(dst + hf * 8192 + swz(r, piece), on ? p : src, on ? 16 : 0);
-            p += next;
-          }
-        }
-      };
-      for (int c = s; c < blocks; c += kTcStages) {
-        const int rows = min(C, seg_rows - c * C);
-        if (c >= kTcStages && !wait_bar(&bars.empty[s], ((c / kTcStages) - 1) & 1, gone)) break;
-        const int64_t f = first + step * c * C;
-        if (!STATE_ONLY) tile(base, qb, P.qs[1], DK / 64, P.kd, f, rows);
-        tile(base + S::KB, kb, P.ks[1], DK / 64, P.kd, f, rows);
-        tile(base + 2 * S::KB, vb, P.vs[1], DV / 64, P.vd, f, rows);
-        mma::cp_commit();
-        mma::cp_wait<0>();
-        tc::fence_smem_to_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.full[s]);
-      }
-      mma::cp_wait<0>();
     }
   }
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  if (warp == 11) tc::tmem_dealloc(tm, 512);
+  if (warp == 19) tc::tmem_dealloc(tm, 512);
   if (tid == 0 && gone_s != 0 && status != nullptr) atomicOr_system(status, TTC_STATUS_MMA_TIMEOUT);
 }
 

@@ -48,9 +48,10 @@ def _status_word() -> int:
 
 def _operand(t: torch.Tensor) -> torch.Tensor:
     """t itself if its head dim is contiguous and its rows start on 16-byte boundaries (a slice of
-    a fused projection, an expanded tensor), else a contiguous copy."""
+    a fused projection), else a contiguous copy (an expanded tensor among these: tensor maps know no
+    stride of 0)."""
     es = t.element_size()
-    ok = t.stride(-1) == 1 and all(n == 1 or s * es % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()))
+    ok = t.stride(-1) == 1 and all(n == 1 or (s > 0 and s * es % 16 == 0) for n, s in zip(t.shape[:-1], t.stride()))
     return _aligned(t if ok else t.contiguous())
 
 
