@@ -45,23 +45,36 @@ struct GN {
   float eps;
 };
 
+// V channels as they lie in memory (one, or 16 bytes), and as floats.
 template <int V, typename T>
-__device__ __forceinline__ void ld_vec(float (&v)[V], const T* p, bool on) {
-  if constexpr (V == 1) {
-    v[0] = on ? ldf(p) : 0.f;
-  } else if constexpr (sizeof(T) == 4) {
-    const float4 a = on ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-  } else {
-    const uint4 a = on ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
-    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+struct Raw {
+  T v;
+  __device__ __forceinline__ void load(const T* p, bool on) { v = on ? *p : T(0.f); }
+  __device__ __forceinline__ void floats(float (&o)[V]) const { o[0] = ldf(&v); }
+};
+template <typename T>
+struct Raw<4, T> {
+  float4 v;
+  __device__ __forceinline__ void load(const T* p, bool on) {
+    v = on ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __device__ __forceinline__ void floats(float (&o)[4]) const { o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w; }
+};
+template <typename T>
+struct Raw<8, T> {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p, bool on) {
+    v = on ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ void floats(float (&o)[8]) const {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(u[i] << 16);
-      v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      o[2 * i] = __uint_as_float(u[i] << 16);
+      o[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
     }
   }
-}
+};
 
 template <int V, typename T>
 __device__ __forceinline__ void st_vec(T* p, const float (&v)[V]) {
@@ -80,10 +93,21 @@ __device__ __forceinline__ void st_vec(T* p, const float (&v)[V]) {
   }
 }
 
+// sigmoid(u).  For bf16 outputs with the approximate exponential and reciprocal, off by a few 2^-22 (the
+// result is rounded to 2^-8); their exact forms are half of the kernels' instructions.
+template <typename T>
+__device__ __forceinline__ float sigmoid(float u) {
+  if constexpr (sizeof(T) == 2) {
+    return __fdividef(1.f, 1.f + __expf(-u));
+  } else {
+    return 1.f / (1.f + expf(-u));
+  }
+}
 // act(u) and act'(u).
+template <typename T>
 __device__ __forceinline__ void act_grad(int act, float u, float& f, float& d) {
   if (act == TTC_ACT_SILU) {
-    const float p = 1.f / (1.f + expf(-u));
+    const float p = sigmoid<T>(u);
     f = u * p;
     d = p * (1.f + u * (1.f - p));
   } else if (act == TTC_ACT_GELU) {
@@ -95,8 +119,9 @@ __device__ __forceinline__ void act_grad(int act, float u, float& f, float& d) {
     d = 1.f;
   }
 }
+template <typename T>
 __device__ __forceinline__ float act_of(int act, float u) {
-  if (act == TTC_ACT_SILU) return u / (1.f + expf(-u));
+  if (act == TTC_ACT_SILU) return u * sigmoid<T>(u);
   if (act == TTC_ACT_GELU) return 0.5f * u * (1.f + erff(u * 0.70710678118654752f));
   return u;
 }
@@ -152,20 +177,34 @@ __global__ void __launch_bounds__(32 * kWarps) group_norm_fwd_kernel(const GN P)
     }
   }
   const T* gate = static_cast<const T*>(P.gate);
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWarps + warp; r < P.rows; r += static_cast<int64_t>(gridDim.x) * kWarps) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
+  Raw<V, T> rx[K], rg[K];
+  auto fetch = [&](int64_t r) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      rx[k].load(static_cast<const T*>(P.x) + r * P.xs + col[k], on[k]);
+      if (gate != nullptr) rg[k].load(gate + r * P.gs + col[k], on[k]);
+    }
+  };
+  int64_t r = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+  constexpr bool AHEAD = K == 1;  // registers for a second row
+  if (AHEAD && r < P.rows) fetch(r);
+  for (; r < P.rows; r += step) {
+    if (!AHEAD) fetch(r);
     float x[K][V], ga[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      ld_vec<V>(x[k], static_cast<const T*>(P.x) + r * P.xs + col[k], on[k]);
-      if (gate != nullptr) ld_vec<V>(ga[k], gate + r * P.gs + col[k], on[k]);
+      rx[k].floats(x[k]);
+      if (gate != nullptr) rg[k].floats(ga[k]);
     }
+    if (AHEAD && r + step < P.rows) fetch(r + step);  // the next row's loads under this one's arithmetic
     const float rstd = normalise<V, K>(x, on, P.seg, inv_n, P.eps);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float z = fmaf(x[k][i] * rstd, w[k][i], b[k][i]);
-        x[k][i] = gate != nullptr ? z * act_of(P.act, ga[k][i]) : act_of(P.act, z);
+        x[k][i] = gate != nullptr ? z * act_of<T>(P.act, ga[k][i]) : act_of<T>(P.act, z);
       }
       if (on[k]) st_vec<V>(static_cast<T*>(P.y) + r * C + col[k], x[k]);
     }
@@ -195,14 +234,29 @@ __global__ void __launch_bounds__(32 * kWarps) group_norm_bwd_kernel(const GN P)
     }
   }
   const T* gate = static_cast<const T*>(P.gate);
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWarps + warp; r < P.rows; r += static_cast<int64_t>(gridDim.x) * kWarps) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
+  Raw<V, T> rx[K], rg[K], rd[K];
+  auto fetch = [&](int64_t r) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      rx[k].load(static_cast<const T*>(P.x) + r * P.xs + col[k], on[k]);
+      rd[k].load(static_cast<const T*>(P.g) + r * C + col[k], on[k]);
+      if (gate != nullptr) rg[k].load(gate + r * P.gs + col[k], on[k]);
+    }
+  };
+  int64_t r = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+  constexpr bool AHEAD = K == 1;  // registers for a second row
+  if (AHEAD && r < P.rows) fetch(r);
+  for (; r < P.rows; r += step) {
+    if (!AHEAD) fetch(r);
     float x[K][V], ga[K][V], g[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      ld_vec<V>(x[k], static_cast<const T*>(P.x) + r * P.xs + col[k], on[k]);
-      ld_vec<V>(g[k], static_cast<const T*>(P.g) + r * C + col[k], on[k]);
-      if (gate != nullptr) ld_vec<V>(ga[k], gate + r * P.gs + col[k], on[k]);
+      rx[k].floats(x[k]);
+      rd[k].floats(g[k]);
+      if (gate != nullptr) rg[k].floats(ga[k]);
     }
+    if (AHEAD && r + step < P.rows) fetch(r + step);  // the next row's loads under this one's arithmetic
     const float rstd = normalise<V, K>(x, on, P.seg, inv_n, P.eps);
     float m1 = 0.f, m2 = 0.f;
 #pragma unroll
@@ -212,11 +266,11 @@ __global__ void __launch_bounds__(32 * kWarps) group_norm_bwd_kernel(const GN P)
         const float xh = x[k][i] * rstd, z = fmaf(xh, w[k][i], b[k][i]);
         float f, d;
         if (gate != nullptr) {
-          act_grad(P.act, ga[k][i], f, d);
+          act_grad<T>(P.act, ga[k][i], f, d);
           ga[k][i] = g[k][i] * z * d;
           g[k][i] *= f;
         } else {
-          act_grad(P.act, z, f, d);
+          act_grad<T>(P.act, z, f, d);
           g[k][i] *= d;
         }
         x[k][i] = xh;
@@ -310,14 +364,14 @@ int seg_of(int n, int v) {
 }
 
 // CTAs along the rows.  About 4 CTAs an SM in all for the backward, whose slabs of dw and db are
-// written and read again (1.2 MB of 537 MB at 16 384 x 4096 bf16); 32 an SM for the forward.
+// written and read again (1.2 MB of 537 MB at 16 384 x 4096 bf16); 8 an SM for the forward.
 int slabs_of(int64_t rows, int groups, int n, int v, int per_sm) {
   const int gpw = 32 / seg_of(n, v);
   const int64_t tiles = (groups + gpw - 1) / gpw;
   const int64_t want = std::max<int64_t>(1, (148LL * per_sm + tiles - 1) / tiles);
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, (rows + kWarps - 1) / kWarps)));
 }
-constexpr int kFwdPerSM = 32, kBwdPerSM = 4;
+constexpr int kFwdPerSM = 8, kBwdPerSM = 4;
 
 bool vec_ok(const void* p, int64_t stride, int v) {
   return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % v == 0);

@@ -1,0 +1,31 @@
+"""Calls of the sequence operators into the library: latency counts for single tokens, so a call is made with
+the raw handle of the current stream, and autograd's machinery only where a gradient is asked for.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib, solver
+
+
+def launch(name, dev, fn, *args) -> None:
+    """fn(*args, stream) on the current stream of ``dev``, which has to be the current device; reported to the
+    solver's kernel timer where one is installed."""
+    if solver._timer is not None:
+        solver._launch(name, dev, fn, *args)
+        return
+    rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        _lib.check(rc)
+
+
+def on_device(dev, f, *args):
+    """f(*args) with ``dev`` as the current device."""
+    if torch._C._cuda_getDevice() == dev.index:
+        return f(*args)
+    with torch.cuda.device(dev):
+        return f(*args)
+
+
+def wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)

@@ -16,7 +16,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .solver import _DTYPES, _aligned, _launch, _ptr
+from ._call import launch, on_device, wants_grad
+from .solver import _DTYPES, _aligned, _ptr
 
 
 def _workspace(nbytes: int, dev) -> torch.Tensor | None:
@@ -90,53 +91,58 @@ def _check_device(name, dev, **tensors):
         raise ValueError(f"ttc_b200 {name} needs CUDA tensors (there is no CPU path)")
 
 
+def _dims(q, v, cu_seqlens):
+    """(T, sequences, H, Hk, dk, dv, dtype code) of the C calls."""
+    B, T, Hk, dk = q.shape
+    return T, B if cu_seqlens is None else cu_seqlens.numel() - 1, v.shape[2], Hk, dk, v.shape[3], _DTYPES[q.dtype]
+
+
+def _forward(q, k, v, log_gamma, scale, initial_state, cu_seqlens, want_state):
+    dev, lib, dims = q.device, _lib.load(), _dims(q, v, cu_seqlens)
+    T, n_seq, H, _, dk, dv, _ = dims
+    o = torch.empty(v.shape, device=dev, dtype=q.dtype)
+    state = torch.empty(n_seq, H, dk, dv, device=dev) if want_state else None
+    nbytes = lib.ttc_decay_attn_workspace(T, n_seq, cu_seqlens is not None, *dims[2:], 0)
+    ws = _workspace(nbytes, dev)
+    launch("ttc_decay_attn_fwd", dev, lib.ttc_decay_attn_fwd, _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v),
+           _ptr(log_gamma), scale, _ptr(initial_state), _ptr(cu_seqlens), *dims, _ptr(o), _ptr(state), _ptr(ws), nbytes,
+           _status_word())
+    return o, state
+
+
+def _backward(q, k, v, log_gamma, scale, initial_state, cu_seqlens, g_o, g_state, want_start):
+    dev, lib, dims = q.device, _lib.load(), _dims(q, v, cu_seqlens)
+    d_q, d_k, d_v = (torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k, v))
+    d_s = torch.empty(initial_state.shape, device=dev) if want_start else None
+    nbytes = lib.ttc_decay_attn_workspace(*dims[:2], cu_seqlens is not None, *dims[2:], 1)
+    ws = _workspace(nbytes, dev)
+    launch("ttc_decay_attn_bwd", dev, lib.ttc_decay_attn_bwd, _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v), _ptr(g_o),
+           _ptr(log_gamma), scale, _ptr(initial_state), _ptr(g_state), _ptr(cu_seqlens), *dims, _ptr(d_q), _ptr(d_k),
+           _ptr(d_v), _ptr(d_s), _ptr(ws), nbytes, _status_word())
+    return d_q, d_k, d_v, d_s
+
+
 class DecayAttentionFunction(torch.autograd.Function):
     """(q, k, v, initial_state) -> (o, last state or None)."""
 
     @staticmethod
     @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, q, k, v, log_gamma, scale, initial_state, cu_seqlens, want_state):
-        dev = q.device
-        q, k, v = _operand(q), _operand(k), _operand(v)
-        B, T, Hk, dk = q.shape
-        H, dv = v.shape[2:]
-        packed = cu_seqlens is not None
-        n_seq = cu_seqlens.numel() - 1 if packed else B
-        lib = _lib.load()
-        dims = (T, n_seq, H, Hk, dk, dv, _DTYPES[q.dtype])
-        with torch.cuda.device(dev):
-            o = torch.empty(B, T, H, dv, device=dev, dtype=q.dtype)
-            state = torch.empty(n_seq, H, dk, dv, device=dev) if want_state else None
-            nbytes = lib.ttc_decay_attn_workspace(T, n_seq, packed, *dims[2:], 0)
-            ws = _workspace(nbytes, dev)
-            _launch("ttc_decay_attn_fwd", dev, lib.ttc_decay_attn_fwd, _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v),
-                    _ptr(log_gamma), scale, _ptr(initial_state), _ptr(cu_seqlens), *dims, _ptr(o), _ptr(state),
-                    _ptr(ws), nbytes, _status_word())
         ctx.save_for_backward(q, k, v, log_gamma, initial_state, cu_seqlens)
-        ctx.dims, ctx.scale = dims, scale
-        return o, state
+        ctx.scale = scale
+        return on_device(q.device, _forward, q, k, v, log_gamma, scale, initial_state, cu_seqlens, want_state)
 
     @staticmethod
     @torch.amp.custom_bwd(device_type="cuda")
     @once_differentiable
     def backward(ctx, g_o, g_state):
         q, k, v, log_gamma, initial_state, cu_seqlens = ctx.saved_tensors
-        dev = q.device
-        packed = cu_seqlens is not None
-        g_o = torch.zeros(v.shape, device=dev, dtype=v.dtype) if g_o is None else _aligned(g_o.to(v.dtype).contiguous())
+        g_o = torch.zeros_like(v) if g_o is None else g_o
+        g_o = _aligned(g_o.to(v.dtype).contiguous())
         g_state = None if g_state is None else g_state.float().contiguous()
-        lib = _lib.load()
-        T, n_seq = ctx.dims[:2]
-        with torch.cuda.device(dev):
-            d_q, d_k, d_v = (torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k, v))
-            d_s = None
-            if initial_state is not None and ctx.needs_input_grad[5]:
-                d_s = torch.empty(initial_state.shape, device=dev)
-            nbytes = lib.ttc_decay_attn_workspace(T, n_seq, packed, *ctx.dims[2:], 1)
-            ws = _workspace(nbytes, dev)
-            _launch("ttc_decay_attn_bwd", dev, lib.ttc_decay_attn_bwd, _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v),
-                    _ptr(g_o), _ptr(log_gamma), ctx.scale, _ptr(initial_state), _ptr(g_state), _ptr(cu_seqlens),
-                    *ctx.dims, _ptr(d_q), _ptr(d_k), _ptr(d_v), _ptr(d_s), _ptr(ws), nbytes, _status_word())
+        want = initial_state is not None and ctx.needs_input_grad[5]
+        d_q, d_k, d_v, d_s = on_device(q.device, _backward, q, k, v, log_gamma, ctx.scale, initial_state, cu_seqlens, g_o,
+                                       g_state, want)
         return d_q, d_k, d_v, None, None, d_s, None, None
 
 
@@ -170,10 +176,13 @@ def decay_attention(q, k, v, log_gamma, scale: float | None = None, initial_stat
         raise ValueError(f"ttc_b200 {name}: initial_state must be float32 [{n_seq},{H},{dk},{dv}], got "
                          f"{initial_state.dtype} {tuple(initial_state.shape)}")
     _check_device(name, q.device, k=k, v=v, log_gamma=log_gamma, initial_state=initial_state, cu_seqlens=cu_seqlens)
-    o, state = DecayAttentionFunction.apply(
-        q, k, v, log_gamma.detach().float().contiguous(), dk ** -0.5 if scale is None else float(scale),
-        None if initial_state is None else initial_state.contiguous(),
-        None if cu_seqlens is None else cu_seqlens.contiguous(), bool(return_state))
+    args = (_operand(q), _operand(k), _operand(v), log_gamma.detach().float().contiguous(),
+            dk ** -0.5 if scale is None else float(scale), None if initial_state is None else initial_state.contiguous(),
+            None if cu_seqlens is None else cu_seqlens.contiguous(), bool(return_state))
+    if wants_grad(q, k, v, initial_state):
+        o, state = DecayAttentionFunction.apply(*args)
+    else:
+        o, state = on_device(q.device, _forward, *args)
     return (o, state) if return_state else o
 
 
@@ -202,10 +211,15 @@ def decay_attention_step(q, k, v, log_gamma, state, slots=None, scale: float | N
     q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
     log_gamma = log_gamma.detach().float().contiguous()
     slots = None if slots is None else slots.contiguous()
-    with torch.cuda.device(dev):
+    scale = dk ** -0.5 if scale is None else float(scale)
+
+    def call():
         o = torch.empty(B, H, dv, device=dev, dtype=q.dtype)
-        _launch("ttc_decay_attn_step", dev, _lib.load().ttc_decay_attn_step, _ptr(q), _ptr(k), _ptr(v),
-                _strides(q, k, v), _ptr(log_gamma), dk ** -0.5 if scale is None else float(scale), _ptr(state),
-                state.stride(0) if n > 1 else H * dk * dv, _ptr(slots), B, n, H, Hk, dk, dv, _DTYPES[q.dtype], _ptr(o))
+        launch("ttc_decay_attn_step", dev, _lib.load().ttc_decay_attn_step, _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v),
+               _ptr(log_gamma), scale, _ptr(state), state.stride(0) if n > 1 else H * dk * dv, _ptr(slots), B, n, H, Hk,
+               dk, dv, _DTYPES[q.dtype], _ptr(o))
+        return o
+
+    o = on_device(dev, call)
     torch.autograd.graph.increment_version(state)
     return o

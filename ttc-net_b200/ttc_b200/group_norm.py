@@ -10,8 +10,9 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
+from ._call import launch, on_device, wants_grad
 from .decay_attention import _workspace
-from .solver import _DTYPES, _launch, _ptr
+from .solver import _DTYPES, _ptr
 
 _ACTS = {"none": _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}
 
@@ -22,49 +23,52 @@ def _rows(t, C):
     return t if t.stride(1) == 1 or C == 1 else t.contiguous()
 
 
+def _dims(x, weight, bias, groups, act, eps):
+    """((rows, groups, channels of a group, act, eps, dtype code), whether the parameters are float32)"""
+    some = weight if weight is not None else bias
+    return ((x.shape[0], groups, x.shape[1] // groups, act, eps, _DTYPES[x.dtype]),
+            int(some is not None and some.dtype == torch.float32))
+
+
+def _forward(x, weight, bias, gate, groups, act, eps):
+    dims, f32 = _dims(x, weight, bias, groups, act, eps)
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    launch("ttc_group_norm_fwd", x.device, _lib.load().ttc_group_norm_fwd, _ptr(x), x.stride(0), _ptr(gate),
+           0 if gate is None else gate.stride(0), _ptr(weight), _ptr(bias), f32, *dims, _ptr(y))
+    return y
+
+
+def _backward(x, weight, bias, gate, groups, act, eps, g, needs):
+    """(dx, dweight, dbias, dgate), None where not needed."""
+    dev, lib = x.device, _lib.load()
+    dims, f32 = _dims(x, weight, bias, groups, act, eps)
+    dx, dw, db, dgate = (torch.empty(t.shape, device=dev, dtype=t.dtype) if need and t is not None else None
+                         for need, t in zip(needs, (x, weight, bias, gate)))
+    nbytes = lib.ttc_group_norm_workspace(*dims[:3], dims[5]) if dw is not None or db is not None else 0
+    ws = _workspace(nbytes, dev)
+    launch("ttc_group_norm_bwd", dev, lib.ttc_group_norm_bwd, _ptr(x), x.stride(0), _ptr(gate),
+           0 if gate is None else gate.stride(0), _ptr(weight), _ptr(bias), f32, _ptr(g), *dims, _ptr(dx), _ptr(dgate),
+           _ptr(dw), _ptr(db), _ptr(ws), nbytes)
+    return dx, dw, db, dgate
+
+
 class GroupNormFunction(torch.autograd.Function):
-    """(x, weight, bias, gate) -> y, all but x may be None."""
+    """(x, weight, bias, gate) -> y for x and gate [rows, C], all but x may be None."""
 
     @staticmethod
     @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, x, weight, bias, gate, groups, act, eps):
-        shape, C, dev = x.shape, x.shape[-1], x.device
-        x2, gate2 = _rows(x, C), None if gate is None else _rows(gate, C)
-        weight, bias = (None if p is None else p.contiguous() for p in (weight, bias))
-        some = weight if weight is not None else bias
-        ctx.dims = (x2.shape[0], groups, C // groups, act, eps, _DTYPES[x.dtype])
-        ctx.param_f32 = int(some is not None and some.dtype == torch.float32)
-        ctx.shape = shape
-        with torch.cuda.device(dev):
-            y = torch.empty(shape, device=dev, dtype=x.dtype)
-            _launch("ttc_group_norm_fwd", dev, _lib.load().ttc_group_norm_fwd, _ptr(x2), x2.stride(0), _ptr(gate2),
-                    0 if gate2 is None else gate2.stride(0), _ptr(weight), _ptr(bias), ctx.param_f32, *ctx.dims, _ptr(y))
-        ctx.save_for_backward(x2, weight, bias, gate2)
-        return y
+        ctx.save_for_backward(x, weight, bias, gate)
+        ctx.how = (groups, act, eps)
+        return on_device(x.device, _forward, x, weight, bias, gate, groups, act, eps)
 
     @staticmethod
     @torch.amp.custom_bwd(device_type="cuda")
     @once_differentiable
     def backward(ctx, g):
-        x, weight, bias, gate = ctx.saved_tensors
-        dev, dtype = x.device, x.dtype
-        g = g.to(dtype).contiguous()
-        lib = _lib.load()
-        with torch.cuda.device(dev):
-            def like(on, t, shape):
-                return torch.empty(shape, device=dev, dtype=t.dtype) if on and t is not None else None
-
-            needs = ctx.needs_input_grad
-            dx = like(needs[0], x, ctx.shape)
-            dw, db = (like(needs[i], p, p.shape if p is not None else None) for i, p in ((1, weight), (2, bias)))
-            dgate = like(needs[3], gate, ctx.shape)
-            rows, groups, n, act, eps, code = ctx.dims
-            nbytes = lib.ttc_group_norm_workspace(rows, groups, n, code) if dw is not None or db is not None else 0
-            ws = _workspace(nbytes, dev)
-            _launch("ttc_group_norm_bwd", dev, lib.ttc_group_norm_bwd, _ptr(x), x.stride(0), _ptr(gate),
-                    0 if gate is None else gate.stride(0), _ptr(weight), _ptr(bias), ctx.param_f32, _ptr(g), rows,
-                    groups, n, act, eps, code, _ptr(dx), _ptr(dgate), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
-        return dx, dw, db, dgate, None, None, None
+        saved = ctx.saved_tensors
+        g = g.to(saved[0].dtype).contiguous()
+        return (*on_device(g.device, _backward, *saved, *ctx.how, g, ctx.needs_input_grad[:4]), None, None, None)
 
 
 def group_norm(x, num_groups: int, weight=None, bias=None, gate=None, activation: str = "none", eps: float = 1e-5):
@@ -92,4 +96,10 @@ def group_norm(x, num_groups: int, weight=None, bias=None, gate=None, activation
             raise ValueError(f"ttc_b200 group_norm: {n} is on {t.device}, x on {x.device}")
     if not x.is_cuda:
         raise ValueError("ttc_b200 group_norm needs CUDA tensors (there is no CPU path)")
-    return GroupNormFunction.apply(x, weight, bias, gate, int(num_groups), _ACTS[activation], float(eps))
+    args = (_rows(x, C), *(None if p is None else p.contiguous() for p in (weight, bias)),
+            None if gate is None else _rows(gate, C), int(num_groups), _ACTS[activation], float(eps))
+    if wants_grad(x, weight, bias, gate):
+        y = GroupNormFunction.apply(*args)
+    else:
+        y = on_device(x.device, _forward, *args)
+    return y.view(x.shape)

@@ -14,7 +14,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .solver import _DTYPES, _launch, _ptr
+from ._call import launch, on_device, wants_grad
+from .solver import _DTYPES, _ptr
 
 
 def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
@@ -49,6 +50,9 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: str = "none
     return f.to(device), magnitude
 
 
+_TWO, _THREE = ctypes.c_int64 * 2, ctypes.c_int64 * 3
+
+
 def _dense(t):
     return t if t.stride(-1) == 1 else t.contiguous()
 
@@ -57,13 +61,11 @@ def _turn(q, k, positions, inv_freq, interleaved, magnitude, inverse):
     dev = q.device
     q, k = _dense(q), None if k is None else _dense(k)
     B, T, H, D = q.shape
-    three = ctypes.c_int64 * 3
-    with torch.cuda.device(dev):
-        outs = [None if t is None else torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k)]
-        _launch("ttc_rotary", dev, _lib.load().ttc_rotary, _ptr(q), three(*q.stride()[:3]), H, _ptr(k),
-                None if k is None else three(*k.stride()[:3]), 0 if k is None else k.shape[2], _ptr(positions),
-                (ctypes.c_int64 * 2)(*positions.stride()), positions.dtype == torch.int64, _ptr(inv_freq), B, T, D,
-                inv_freq.numel(), interleaved, inverse, magnitude, _DTYPES[q.dtype], _ptr(outs[0]), _ptr(outs[1]))
+    outs = [None if t is None else torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k)]
+    launch("ttc_rotary", dev, _lib.load().ttc_rotary, _ptr(q), _THREE(*q.stride()[:3]), H, _ptr(k),
+           None if k is None else _THREE(*k.stride()[:3]), 0 if k is None else k.shape[2], _ptr(positions),
+           _TWO(*positions.stride()), positions.dtype == torch.int64, _ptr(inv_freq), B, T, D, inv_freq.numel(),
+           interleaved, inverse, magnitude, _DTYPES[q.dtype], _ptr(outs[0]), _ptr(outs[1]))
     return outs
 
 
@@ -76,7 +78,7 @@ class RotaryFunction(torch.autograd.Function):
         ctx.save_for_backward(positions, inv_freq)
         ctx.how = (interleaved, magnitude)
         ctx.like = tuple(None if t is None else (t.shape, t.dtype, t.device) for t in (q, k))
-        return tuple(_turn(q, k, positions, inv_freq, *ctx.how, False))
+        return tuple(on_device(q.device, _turn, q, k, positions, inv_freq, *ctx.how, False))
 
     @staticmethod
     @torch.amp.custom_bwd(device_type="cuda")
@@ -89,7 +91,7 @@ class RotaryFunction(torch.autograd.Function):
                 shape, dtype, dev = like
                 g = torch.zeros(shape, dtype=dtype, device=dev) if g is None else g.to(dtype)
             gs.append(g)
-        return (*_turn(*gs, positions, inv_freq, *ctx.how, True), None, None, None, None)
+        return (*on_device(gs[0].device, _turn, *gs, positions, inv_freq, *ctx.how, True), None, None, None, None)
 
 
 def rotary(q, k, positions, inv_freq, interleaved: bool = False, magnitude: float = 1.0):
@@ -120,5 +122,8 @@ def rotary(q, k, positions, inv_freq, interleaved: bool = False, magnitude: floa
             raise ValueError(f"ttc_b200 rotary: {n} is on {t.device}, q on {q.device}")
     if not q.is_cuda:
         raise ValueError("ttc_b200 rotary needs CUDA tensors (there is no CPU path)")
-    return RotaryFunction.apply(q, k, positions.expand(B, T), inv_freq.detach().contiguous(), bool(interleaved),
-                                float(magnitude))
+    args = (q, k, positions if positions.shape == (B, T) else positions.expand(B, T), inv_freq.detach().contiguous(),
+            bool(interleaved), float(magnitude))
+    if wants_grad(q, k):
+        return RotaryFunction.apply(*args)
+    return tuple(on_device(q.device, _turn, *args, False))
