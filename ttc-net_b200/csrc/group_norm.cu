@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <cstdio>
+#include <type_traits>
 
 #include "lqr_common.cuh"
 #include "ttc_b200.h"
@@ -45,12 +46,61 @@ struct GN {
   float eps;
 };
 
-// V channels as they lie in memory (one, or 16 bytes), and as floats.
+// One or two neighbouring channels in fp32; two at a time with the packed instructions (the kernels
+// are bound by instructions, not by memory, where each channel takes its own).
+template <int V>
+struct ElemOf {
+  using type = float2;
+};
+template <>
+struct ElemOf<1> {
+  using type = float;
+};
+__device__ __forceinline__ float add(float a, float b) { return a + b; }
+__device__ __forceinline__ float mul(float a, float b) { return a * b; }
+__device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ uint64_t pair(float2 a) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t r) {
+  float2 a;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
+  return a;
+}
+__device__ __forceinline__ float2 add(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)));
+  return unpair(r);
+}
+__device__ __forceinline__ float2 mul(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)));
+  return unpair(r);
+}
+__device__ __forceinline__ float2 fma_(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)), "l"(pair(c)));
+  return unpair(r);
+}
+template <typename E>
+__device__ __forceinline__ E all(float a) {
+  if constexpr (sizeof(E) == 4) {
+    return a;
+  } else {
+    return make_float2(a, a);
+  }
+}
+__device__ __forceinline__ float both(float a) { return a; }
+__device__ __forceinline__ float both(float2 a) { return a.x + a.y; }
+
+// V channels as they lie in memory (one, or 16 bytes), and as numbers.
 template <int V, typename T>
 struct Raw {
   T v;
   __device__ __forceinline__ void load(const T* p, bool on) { v = on ? *p : T(0.f); }
-  __device__ __forceinline__ void floats(float (&o)[V]) const { o[0] = ldf(&v); }
+  __device__ __forceinline__ void get(float (&o)[1]) const { o[0] = ldf(&v); }
 };
 template <typename T>
 struct Raw<4, T> {
@@ -58,7 +108,7 @@ struct Raw<4, T> {
   __device__ __forceinline__ void load(const T* p, bool on) {
     v = on ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  __device__ __forceinline__ void floats(float (&o)[4]) const { o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w; }
+  __device__ __forceinline__ void get(float2 (&o)[2]) const { o[0] = make_float2(v.x, v.y), o[1] = make_float2(v.z, v.w); }
 };
 template <typename T>
 struct Raw<8, T> {
@@ -66,35 +116,32 @@ struct Raw<8, T> {
   __device__ __forceinline__ void load(const T* p, bool on) {
     v = on ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
   }
-  __device__ __forceinline__ void floats(float (&o)[8]) const {
+  __device__ __forceinline__ void get(float2 (&o)[4]) const {
     const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      o[2 * i] = __uint_as_float(u[i] << 16);
-      o[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-    }
+    for (int i = 0; i < 4; ++i) o[i] = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
   }
 };
 
-template <int V, typename T>
-__device__ __forceinline__ void st_vec(T* p, const float (&v)[V]) {
-  if constexpr (V == 1) {
-    stf(p, v[0]);
-  } else if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
-    uint32_t u[4];
+template <typename T>
+__device__ __forceinline__ void put(T* p, const float (&v)[1]) {
+  stf(p, v[0]);
+}
+__device__ __forceinline__ void put(float* p, const float2 (&v)[2]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+}
+__device__ __forceinline__ void put(__nv_bfloat16* p, const float2 (&v)[4]) {
+  uint32_t u[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-      u[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[i].x, v[i].y);
+    u[i] = *reinterpret_cast<const uint32_t*>(&h);
   }
+  *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
 }
 
 // sigmoid(u).  For bf16 outputs with the approximate exponential and reciprocal, off by a few 2^-22 (the
-// result is rounded to 2^-8); their exact forms are half of the kernels' instructions.
+// result is rounded to 2^-8); their exact forms were half of the kernels' instructions.
 template <typename T>
 __device__ __forceinline__ float sigmoid(float u) {
   if constexpr (sizeof(T) == 2) {
@@ -103,31 +150,74 @@ __device__ __forceinline__ float sigmoid(float u) {
     return 1.f / (1.f + expf(-u));
   }
 }
-// act(u) and act'(u).
 template <typename T>
-__device__ __forceinline__ void act_grad(int act, float u, float& f, float& d) {
-  if (act == TTC_ACT_SILU) {
-    const float p = sigmoid<T>(u);
-    f = u * p;
-    d = p * (1.f + u * (1.f - p));
-  } else if (act == TTC_ACT_GELU) {
-    const float c = 0.5f * (1.f + erff(u * 0.70710678118654752f));
-    f = u * c;
-    d = c + u * 0.3989422804014327f * expf(-0.5f * u * u);
+__device__ __forceinline__ float2 sigmoid2(float2 u) {
+  return make_float2(sigmoid<T>(u.x), sigmoid<T>(u.y));
+}
+template <typename T>
+__device__ __forceinline__ float sigmoid2(float u) {
+  return sigmoid<T>(u);
+}
+// Phi(u) and the normal density.
+__device__ __forceinline__ float cdf(float u) { return 0.5f * (1.f + erff(u * 0.70710678118654752f)); }
+__device__ __forceinline__ float2 cdf(float2 u) { return make_float2(cdf(u.x), cdf(u.y)); }
+__device__ __forceinline__ float pdf(float u) { return 0.3989422804014327f * expf(-0.5f * u * u); }
+__device__ __forceinline__ float2 pdf(float2 u) { return make_float2(pdf(u.x), pdf(u.y)); }
+
+// f = act(u) and d = act'(u).
+template <int ACT, typename T, typename E>
+__device__ __forceinline__ void act_grad(E u, E& f, E& d) {
+  if constexpr (ACT == TTC_ACT_SILU) {
+    const E p = sigmoid2<T>(u);
+    f = mul(u, p);
+    // p (1 + u (1 - p)) = p + f (1 - p)
+    d = fma_(f, fma_(p, all<E>(-1.f), all<E>(1.f)), p);
+  } else if constexpr (ACT == TTC_ACT_GELU) {
+    const E c = cdf(u);
+    f = mul(u, c);
+    d = fma_(u, pdf(u), c);
   } else {
     f = u;
-    d = 1.f;
+    d = all<E>(1.f);
   }
 }
-template <typename T>
-__device__ __forceinline__ float act_of(int act, float u) {
-  if (act == TTC_ACT_SILU) return u * sigmoid<T>(u);
-  if (act == TTC_ACT_GELU) return 0.5f * u * (1.f + erff(u * 0.70710678118654752f));
+template <int ACT, typename T, typename E>
+__device__ __forceinline__ E act_of(E u) {
+  if constexpr (ACT == TTC_ACT_SILU) return mul(u, sigmoid2<T>(u));
+  if constexpr (ACT == TTC_ACT_GELU) return mul(u, cdf(u));
   return u;
 }
+// f(activation, whether there is a gate), both as compile-time constants: one branch for a whole row.
+template <typename F>
+__device__ __forceinline__ void with_kind(int act, bool gated, F&& f) {
+  using std::integral_constant;
+  if (act == TTC_ACT_SILU) {
+    if (gated)
+      f(integral_constant<int, TTC_ACT_SILU>{}, std::true_type{});
+    else
+      f(integral_constant<int, TTC_ACT_SILU>{}, std::false_type{});
+  } else if (act == TTC_ACT_GELU) {
+    if (gated)
+      f(integral_constant<int, TTC_ACT_GELU>{}, std::true_type{});
+    else
+      f(integral_constant<int, TTC_ACT_GELU>{}, std::false_type{});
+  } else {
+    if (gated)
+      f(integral_constant<int, TTC_ACT_NONE>{}, std::true_type{});
+    else
+      f(integral_constant<int, TTC_ACT_NONE>{}, std::false_type{});
+  }
+}
 
+// Sum over the SEG lanes of a group (SEG = 0: `seg` of them).
+template <int SEG>
 __device__ __forceinline__ float seg_sum(float v, int seg) {
-  for (int o = seg >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (SEG > 0) {
+#pragma unroll
+    for (int o = SEG / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  } else {
+    for (int o = seg >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  }
   return v;
 }
 
@@ -137,45 +227,70 @@ __device__ __forceinline__ float param(const void* p, int f32, bool bf16, int64_
 }
 
 // Deviations from the mean (0 beyond the group) and rstd of the group held in x.
-template <int V, int K>
-__device__ __forceinline__ float normalise(float (&x)[K][V], const bool (&on)[K], int seg, float inv_n, float eps) {
-  float s = 0.f;
+template <int SEG, int K, typename E, int N>
+__device__ __forceinline__ float normalise(E (&x)[K][N], const bool (&on)[K], int seg, float inv_n, float eps) {
+  E s = all<E>(0.f);
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int i = 0; i < V; ++i) s += x[k][i];
-  const float mean = seg_sum(s, seg) * inv_n;
-  float q = 0.f;
+    for (int i = 0; i < N; ++i) s = add(s, x[k][i]);
+  const E mean = all<E>(-seg_sum<SEG>(both(s), seg) * inv_n);
+  E q = all<E>(0.f);
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      x[k][i] = on[k] ? x[k][i] - mean : 0.f;
-      q = fmaf(x[k][i], x[k][i], q);
+    for (int i = 0; i < N; ++i) {
+      x[k][i] = on[k] ? add(x[k][i], mean) : all<E>(0.f);
+      q = fma_(x[k][i], x[k][i], q);
     }
-  return rsqrtf(seg_sum(q, seg) * inv_n + eps);
+  return rsqrtf(seg_sum<SEG>(both(q), seg) * inv_n + eps);
 }
 
-template <typename T, int V, int K>
+// Weight and bias of a CTA's columns, and where a lane finds its own: element i of vector k at [k N + i][lane].
+template <int K, typename E, int N>
+struct Params {
+  E w[K * N][32], b[K * N][32];
+  template <typename T>
+  __device__ __forceinline__ void load(const GN& P, const bool (&on)[K], const int64_t (&col)[K]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int PER = sizeof(E) / 4;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (warp == (k * N + i) % kWarps) {
+          float v[2][PER];
+#pragma unroll
+          for (int e = 0; e < PER; ++e) {
+            v[0][e] = on[k] ? param(P.w, P.w_f32, sizeof(T) == 2, col[k] + i * PER + e, 1.f) : 0.f;
+            v[1][e] = on[k] ? param(P.b, P.w_f32, sizeof(T) == 2, col[k] + i * PER + e, 0.f) : 0.f;
+          }
+          w[k * N + i][lane] = *reinterpret_cast<const E*>(v[0]);
+          b[k * N + i][lane] = *reinterpret_cast<const E*>(v[1]);
+        }
+    __syncthreads();
+  }
+};
+
+template <typename T, int V, int K, int SEG>
 __global__ void __launch_bounds__(32 * kWarps) group_norm_fwd_kernel(const GN P) {
+  using E = typename ElemOf<V>::type;
+  constexpr int N = V == 1 ? 1 : V / 2;
+  __shared__ __align__(16) Params<K, E, N> par;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int ls = lane % P.seg, group = blockIdx.y * (32 / P.seg) + lane / P.seg;
+  const int seg = SEG > 0 ? SEG : P.seg;
+  const int ls = lane % seg, group = blockIdx.y * (32 / seg) + lane / seg;
   const int64_t C = static_cast<int64_t>(P.groups) * P.n;
   const float inv_n = 1.f / P.n;
   bool on[K];
   int64_t col[K];
-  float w[K][V], b[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int c = (ls + k * P.seg) * V;
+    const int c = (ls + k * seg) * V;
     on[k] = group < P.groups && c < P.n;
     col[k] = on[k] ? static_cast<int64_t>(group) * P.n + c : 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      w[k][i] = on[k] ? param(P.w, P.w_f32, sizeof(T) == 2, col[k] + i, 1.f) : 0.f;
-      b[k][i] = on[k] ? param(P.b, P.w_f32, sizeof(T) == 2, col[k] + i, 0.f) : 0.f;
-    }
   }
+  par.template load<T>(P, on, col);
   const T* gate = static_cast<const T*>(P.gate);
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
   Raw<V, T> rx[K], rg[K];
@@ -186,53 +301,60 @@ __global__ void __launch_bounds__(32 * kWarps) group_norm_fwd_kernel(const GN P)
       if (gate != nullptr) rg[k].load(gate + r * P.gs + col[k], on[k]);
     }
   };
-  int64_t r = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
   constexpr bool AHEAD = K == 1;  // registers for a second row
+  int64_t r = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
   if (AHEAD && r < P.rows) fetch(r);
   for (; r < P.rows; r += step) {
     if (!AHEAD) fetch(r);
-    float x[K][V], ga[K][V];
+    E x[K][N], ga[K][N];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      rx[k].floats(x[k]);
-      if (gate != nullptr) rg[k].floats(ga[k]);
+      rx[k].get(x[k]);
+      if (gate != nullptr) rg[k].get(ga[k]);
     }
     if (AHEAD && r + step < P.rows) fetch(r + step);  // the next row's loads under this one's arithmetic
-    const float rstd = normalise<V, K>(x, on, P.seg, inv_n, P.eps);
+    const E rstd = all<E>(normalise<SEG>(x, on, seg, inv_n, P.eps));
+    with_kind(P.act, gate != nullptr, [&](auto act, auto gated) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
+      for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float z = fmaf(x[k][i] * rstd, w[k][i], b[k][i]);
-        x[k][i] = gate != nullptr ? z * act_of<T>(P.act, ga[k][i]) : act_of<T>(P.act, z);
-      }
-      if (on[k]) st_vec<V>(static_cast<T*>(P.y) + r * C + col[k], x[k]);
-    }
+        for (int i = 0; i < N; ++i) {
+          const E z = fma_(mul(x[k][i], rstd), par.w[k * N + i][lane], par.b[k * N + i][lane]);
+          if constexpr (decltype(gated)::value)
+            x[k][i] = mul(z, act_of<decltype(act)::value, T>(ga[k][i]));
+          else
+            x[k][i] = act_of<decltype(act)::value, T>(z);
+        }
+    });
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (on[k]) put(static_cast<T*>(P.y) + r * C + col[k], x[k]);
   }
 }
 
-template <typename T, int V, int K>
-__global__ void __launch_bounds__(32 * kWarps) group_norm_bwd_kernel(const GN P) {
-  __shared__ float red[kWarps][32 * K * V];
+template <typename T, int V, int K, int SEG>
+__global__ void __launch_bounds__(32 * kWarps, K == 1 ? 2 : 1) group_norm_bwd_kernel(const GN P) {
+  using E = typename ElemOf<V>::type;
+  constexpr int N = V == 1 ? 1 : V / 2;
+  __shared__ __align__(16) Params<K, E, N> par;
+  __shared__ __align__(16) E red[kWarps][K * N][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int ls = lane % P.seg, group = blockIdx.y * (32 / P.seg) + lane / P.seg;
+  const int seg = SEG > 0 ? SEG : P.seg;
+  const int ls = lane % seg, group = blockIdx.y * (32 / seg) + lane / seg;
   const int64_t C = static_cast<int64_t>(P.groups) * P.n;
   const float inv_n = 1.f / P.n;
   bool on[K];
   int64_t col[K];
-  float w[K][V], b[K][V], dw[K][V], db[K][V];
+  E dw[K][N], db[K][N];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int c = (ls + k * P.seg) * V;
+    const int c = (ls + k * seg) * V;
     on[k] = group < P.groups && c < P.n;
     col[k] = on[k] ? static_cast<int64_t>(group) * P.n + c : 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      w[k][i] = on[k] ? param(P.w, P.w_f32, sizeof(T) == 2, col[k] + i, 1.f) : 0.f;
-      b[k][i] = on[k] ? param(P.b, P.w_f32, sizeof(T) == 2, col[k] + i, 0.f) : 0.f;
-      dw[k][i] = db[k][i] = 0.f;
-    }
+    for (int i = 0; i < N; ++i) dw[k][i] = db[k][i] = all<E>(0.f);
   }
+  par.template load<T>(P, on, col);
   const T* gate = static_cast<const T*>(P.gate);
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
   Raw<V, T> rx[K], rg[K], rd[K];
@@ -249,67 +371,75 @@ __global__ void __launch_bounds__(32 * kWarps) group_norm_bwd_kernel(const GN P)
   if (AHEAD && r < P.rows) fetch(r);
   for (; r < P.rows; r += step) {
     if (!AHEAD) fetch(r);
-    float x[K][V], ga[K][V], g[K][V];
+    E x[K][N], ga[K][N], g[K][N];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      rx[k].floats(x[k]);
-      rd[k].floats(g[k]);
-      if (gate != nullptr) rg[k].floats(ga[k]);
+      rx[k].get(x[k]);
+      rd[k].get(g[k]);
+      if (gate != nullptr) rg[k].get(ga[k]);
     }
     if (AHEAD && r + step < P.rows) fetch(r + step);  // the next row's loads under this one's arithmetic
-    const float rstd = normalise<V, K>(x, on, P.seg, inv_n, P.eps);
-    float m1 = 0.f, m2 = 0.f;
+    const float rs = normalise<SEG>(x, on, seg, inv_n, P.eps);
+    const E rstd = all<E>(rs);
+    // beyond the group g is 0, and so is every sum's part
+    E s1 = all<E>(0.f), s2 = all<E>(0.f);
+    with_kind(P.act, gate != nullptr, [&](auto act, auto gated) {
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+      for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float xh = x[k][i] * rstd, z = fmaf(xh, w[k][i], b[k][i]);
-        float f, d;
-        if (gate != nullptr) {
-          act_grad<T>(P.act, ga[k][i], f, d);
-          ga[k][i] = g[k][i] * z * d;
-          g[k][i] *= f;
-        } else {
-          act_grad<T>(P.act, z, f, d);
-          g[k][i] *= d;
+        for (int i = 0; i < N; ++i) {
+          const E w = par.w[k * N + i][lane];
+          x[k][i] = mul(x[k][i], rstd);
+          const E z = fma_(x[k][i], w, par.b[k * N + i][lane]);
+          E f, d;
+          if constexpr (decltype(gated)::value) {
+            act_grad<decltype(act)::value, T>(ga[k][i], f, d);
+            ga[k][i] = mul(mul(g[k][i], z), d);
+            g[k][i] = mul(g[k][i], f);
+          } else {
+            act_grad<decltype(act)::value, T>(z, f, d);
+            g[k][i] = mul(g[k][i], d);
+          }
+          dw[k][i] = fma_(g[k][i], x[k][i], dw[k][i]);
+          db[k][i] = add(db[k][i], g[k][i]);
+          g[k][i] = mul(g[k][i], w);
+          s1 = add(s1, g[k][i]);
+          s2 = fma_(g[k][i], x[k][i], s2);
         }
-        x[k][i] = xh;
-        if (on[k]) {
-          dw[k][i] = fmaf(g[k][i], xh, dw[k][i]);
-          db[k][i] += g[k][i];
-        }
-        g[k][i] = on[k] ? g[k][i] * w[k][i] : 0.f;
-        m1 += g[k][i];
-        m2 = fmaf(g[k][i], xh, m2);
-      }
-    m1 = seg_sum(m1, P.seg) * inv_n;
-    m2 = seg_sum(m2, P.seg) * inv_n;
+    });
+    const E m1 = all<E>(-seg_sum<SEG>(both(s1), seg) * inv_n), m2 = all<E>(-seg_sum<SEG>(both(s2), seg) * inv_n);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) x[k][i] = rstd * (g[k][i] - m1 - x[k][i] * m2);
+      for (int i = 0; i < N; ++i) x[k][i] = mul(rstd, fma_(x[k][i], m2, add(g[k][i], m1)));
       if (on[k]) {
-        if (P.dx != nullptr) st_vec<V>(static_cast<T*>(P.dx) + r * C + col[k], x[k]);
-        if (P.dgate != nullptr) st_vec<V>(static_cast<T*>(P.dgate) + r * C + col[k], ga[k]);
+        if (P.dx != nullptr) put(static_cast<T*>(P.dx) + r * C + col[k], x[k]);
+        if (P.dgate != nullptr) put(static_cast<T*>(P.dgate) + r * C + col[k], ga[k]);
       }
     }
   }
   if (P.partial == nullptr) return;
+  constexpr int PER = sizeof(E) / 4;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) red[warp][(k * V + i) * 32 + lane] = which ? db[k][i] : dw[k][i];
+      for (int i = 0; i < N; ++i) red[warp][k * N + i][lane] = which ? db[k][i] : dw[k][i];
     __syncthreads();
-    for (int e = warp; e < K * V; e += kWarps) {
-      float s = 0.f;
+    for (int e = warp; e < K * N; e += kWarps) {
+      E s = all<E>(0.f);
 #pragma unroll
-      for (int u = 0; u < kWarps; ++u) s += red[u][e * 32 + lane];
-      const int c = (ls + (e / V) * P.seg) * V;  // this lane's vector number e / V
-      if (group < P.groups && c < P.n)
-        P.partial[(static_cast<int64_t>(blockIdx.x) * 2 + which) * C + static_cast<int64_t>(group) * P.n + c + e % V] = s;
+      for (int u = 0; u < kWarps; ++u) s = add(s, red[u][e][lane]);
+      const int c = (ls + (e / N) * seg) * V;  // this lane's vector number e / N
+      if (group < P.groups && c < P.n) {
+        float* o = P.partial + (static_cast<int64_t>(blockIdx.x) * 2 + which) * C + static_cast<int64_t>(group) * P.n + c +
+                   (e % N) * PER;
+        const float* v = reinterpret_cast<const float*>(&s);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) o[j] = v[j];
+      }
     }
   }
 }
@@ -363,15 +493,16 @@ int seg_of(int n, int v) {
   return seg;
 }
 
-// CTAs along the rows.  About 4 CTAs an SM in all for the backward, whose slabs of dw and db are
-// written and read again (1.2 MB of 537 MB at 16 384 x 4096 bf16); 8 an SM for the forward.
+// CTAs along the rows: as many as are resident at once, 2 an SM for the backward, whose slabs of dw and db are
+// written and read again (0.6 MB beside 671 MB at 16 384 x 4096 bf16; with 3 an SM, at 80 registers, it took 161 us against 134), 6 an SM for the forward.
 int slabs_of(int64_t rows, int groups, int n, int v, int per_sm) {
   const int gpw = 32 / seg_of(n, v);
   const int64_t tiles = (groups + gpw - 1) / gpw;
-  const int64_t want = std::max<int64_t>(1, (148LL * per_sm + tiles - 1) / tiles);
+  // not one CTA more than fit at once: a last wave of a few would cost as much as a full one
+  const int64_t want = std::max<int64_t>(1, 148LL * per_sm / tiles);
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, (rows + kWarps - 1) / kWarps)));
 }
-constexpr int kFwdPerSM = 8, kBwdPerSM = 4;
+constexpr int kFwdPerSM = 6, kBwdPerSM = 2;
 
 bool vec_ok(const void* p, int64_t stride, int v) {
   return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % v == 0);
@@ -388,24 +519,31 @@ int run(GN P, bool backward, void* dw, void* db, cudaStream_t st) {
   const int gpw = 32 / P.seg, per_lane = (P.n + P.seg * v - 1) / (P.seg * v);
   const int slabs = slabs_of(P.rows, P.groups, P.n, v, backward ? kBwdPerSM : kFwdPerSM);
   const dim3 grid(slabs, (P.groups + gpw - 1) / gpw);
-#define TTC_GN(V, K)                                                  \
-  do {                                                                \
-    if (backward)                                                     \
-      group_norm_bwd_kernel<T, V, K><<<grid, 32 * kWarps, 0, st>>>(P); \
-    else                                                              \
-      group_norm_fwd_kernel<T, V, K><<<grid, 32 * kWarps, 0, st>>>(P); \
+#define TTC_GN(V, K, SEG)                                                  \
+  do {                                                                     \
+    if (backward)                                                          \
+      group_norm_bwd_kernel<T, V, K, SEG><<<grid, 32 * kWarps, 0, st>>>(P); \
+    else                                                                   \
+      group_norm_fwd_kernel<T, V, K, SEG><<<grid, 32 * kWarps, 0, st>>>(P); \
   } while (0)
   if (vec) {
-    if (per_lane == 1)
-      TTC_GN(VT, 1);
-    else if (per_lane <= 4)
-      TTC_GN(VT, 4);
-    else if constexpr (VT == 4)
-      TTC_GN(VT, 8);
+    if (per_lane == 1) {
+      switch (P.seg) {
+        case 4: TTC_GN(VT, 1, 4); break;
+        case 8: TTC_GN(VT, 1, 8); break;
+        case 16: TTC_GN(VT, 1, 16); break;
+        case 32: TTC_GN(VT, 1, 32); break;
+        default: TTC_GN(VT, 1, 0);
+      }
+    } else if (per_lane <= 4) {
+      TTC_GN(VT, 4, 32);
+    } else if constexpr (VT == 4) {
+      TTC_GN(VT, 8, 32);
+    }
   } else if (per_lane <= 4) {
-    TTC_GN(1, 4);
+    TTC_GN(1, 4, 0);
   } else {
-    TTC_GN(1, 32);
+    TTC_GN(1, 32, 32);
   }
 #undef TTC_GN
   if (int rc = launched(backward ? "group_norm_bwd_kernel launch" : "group_norm_fwd_kernel launch")) return rc;

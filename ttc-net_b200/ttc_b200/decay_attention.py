@@ -51,36 +51,47 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
     """t itself if its head dim is contiguous and its rows start on 16-byte boundaries (a slice of
     a fused projection), else a contiguous copy (an expanded tensor among these: tensor maps know no
     stride of 0)."""
+    if t.is_contiguous():
+        return _aligned(t)
     es = t.element_size()
     ok = t.stride(-1) == 1 and all(n == 1 or (s > 0 and s * es % 16 == 0) for n, s in zip(t.shape[:-1], t.stride()))
     return _aligned(t if ok else t.contiguous())
 
 
-def _strides(*tensors):
-    flat = [0 if n == 1 else s for t in tensors for n, s in zip(t.shape[:-1], t.stride())]
-    return (ctypes.c_int64 * len(flat))(*flat)
+_SIX, _NINE = ctypes.c_int64 * 6, ctypes.c_int64 * 9
+
+
+def _strides(t: torch.Tensor):
+    """Strides of the dims before the head dim; those of a dim of one element do not matter and may be odd."""
+    return t.stride()[:-1] if t.is_contiguous() else [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride())]
 
 
 def _check_qkv(name, q, k, v, log_gamma, lead):
     """Types, devices and shapes of q, k [*lead, Hk, dk], v [*lead, H, dv], log_gamma [H]."""
-    for t, n in ((q, "q"), (k, "k"), (v, "v")):
-        if t.dtype not in _DTYPES:
-            raise TypeError(f"ttc_b200 {name} supports float32 and bfloat16, got {t.dtype} for {n}")
-        if t.dim() != lead + 2:
-            raise ValueError(f"ttc_b200 {name}: {n} must have {lead + 2} dimensions, got {tuple(t.shape)}")
-    if not q.dtype == k.dtype == v.dtype:
-        raise TypeError(f"ttc_b200 {name}: q, k and v must have one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
-    if q.shape != k.shape or q.shape[:lead] != v.shape[:lead]:
-        raise ValueError(f"ttc_b200 {name}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
-    Hk, dk = q.shape[lead:]
-    H, dv = v.shape[lead:]
+    qs, vs, dt = q.shape, v.shape, q.dtype
+    if not (dt in _DTYPES and k.dtype == dt and v.dtype == dt and len(qs) == lead + 2 and qs == k.shape
+            and len(vs) == lead + 2 and qs[:lead] == vs[:lead]):
+        for t, n in ((q, "q"), (k, "k"), (v, "v")):
+            if t.dtype not in _DTYPES:
+                raise TypeError(f"ttc_b200 {name} supports float32 and bfloat16, got {t.dtype} for {n}")
+            if t.dim() != lead + 2:
+                raise ValueError(f"ttc_b200 {name}: {n} must have {lead + 2} dimensions, got {tuple(t.shape)}")
+        if not q.dtype == k.dtype == v.dtype:
+            raise TypeError(f"ttc_b200 {name}: q, k and v must have one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
+        raise ValueError(f"ttc_b200 {name}: q {tuple(qs)}, k {tuple(k.shape)} and v {tuple(vs)} do not match")
+    Hk, dk = qs[lead:]
+    H, dv = vs[lead:]
     if Hk < 1 or H % Hk:
         raise ValueError(f"ttc_b200 {name}: {H} value heads are not a multiple of {Hk} key heads")
-    if tuple(log_gamma.shape) != (H,) or not log_gamma.dtype.is_floating_point:
+    if log_gamma.shape != (H,) or not log_gamma.dtype.is_floating_point:
         raise ValueError(f"ttc_b200 {name}: log_gamma must be [{H}] floating point, got {tuple(log_gamma.shape)}")
-    if torch.is_grad_enabled() and log_gamma.requires_grad:
+    if log_gamma.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"ttc_b200 {name}: the decays are fixed, log_gamma must not require a gradient")
     return H, Hk, dk, dv
+
+
+def _decays(log_gamma):
+    return log_gamma if log_gamma.dtype == torch.float32 and log_gamma.is_contiguous() else log_gamma.float().contiguous()
 
 
 def _check_device(name, dev, **tensors):
@@ -104,8 +115,8 @@ def _forward(q, k, v, log_gamma, scale, initial_state, cu_seqlens, want_state):
     state = torch.empty(n_seq, H, dk, dv, device=dev) if want_state else None
     nbytes = lib.ttc_decay_attn_workspace(T, n_seq, cu_seqlens is not None, *dims[2:], 0)
     ws = _workspace(nbytes, dev)
-    launch("ttc_decay_attn_fwd", dev, lib.ttc_decay_attn_fwd, _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v),
-           _ptr(log_gamma), scale, _ptr(initial_state), _ptr(cu_seqlens), *dims, _ptr(o), _ptr(state), _ptr(ws), nbytes,
+    launch("ttc_decay_attn_fwd", dev, lib.ttc_decay_attn_fwd, _ptr(q), _ptr(k), _ptr(v),
+           _NINE(*_strides(q), *_strides(k), *_strides(v)), _ptr(log_gamma), scale, _ptr(initial_state), _ptr(cu_seqlens), *dims, _ptr(o), _ptr(state), _ptr(ws), nbytes,
            _status_word())
     return o, state
 
@@ -116,10 +127,19 @@ def _backward(q, k, v, log_gamma, scale, initial_state, cu_seqlens, g_o, g_state
     d_s = torch.empty(initial_state.shape, device=dev) if want_start else None
     nbytes = lib.ttc_decay_attn_workspace(*dims[:2], cu_seqlens is not None, *dims[2:], 1)
     ws = _workspace(nbytes, dev)
-    launch("ttc_decay_attn_bwd", dev, lib.ttc_decay_attn_bwd, _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v), _ptr(g_o),
-           _ptr(log_gamma), scale, _ptr(initial_state), _ptr(g_state), _ptr(cu_seqlens), *dims, _ptr(d_q), _ptr(d_k),
+    launch("ttc_decay_attn_bwd", dev, lib.ttc_decay_attn_bwd, _ptr(q), _ptr(k), _ptr(v),
+           _NINE(*_strides(q), *_strides(k), *_strides(v)), _ptr(g_o), _ptr(log_gamma), scale, _ptr(initial_state), _ptr(g_state), _ptr(cu_seqlens), *dims, _ptr(d_q), _ptr(d_k),
            _ptr(d_v), _ptr(d_s), _ptr(ws), nbytes, _status_word())
     return d_q, d_k, d_v, d_s
+
+
+def _step(q, k, v, log_gamma, scale, state, slot_stride, slots, dims):
+    dev = q.device
+    o = torch.empty(v.shape, device=dev, dtype=q.dtype)
+    launch("ttc_decay_attn_step", dev, _lib.load().ttc_decay_attn_step, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+           _SIX(*_strides(q), *_strides(k), *_strides(v)), log_gamma.data_ptr(), scale, state.data_ptr(), slot_stride,
+           _ptr(slots), *dims, o.data_ptr())
+    return o
 
 
 class DecayAttentionFunction(torch.autograd.Function):
@@ -176,7 +196,7 @@ def decay_attention(q, k, v, log_gamma, scale: float | None = None, initial_stat
         raise ValueError(f"ttc_b200 {name}: initial_state must be float32 [{n_seq},{H},{dk},{dv}], got "
                          f"{initial_state.dtype} {tuple(initial_state.shape)}")
     _check_device(name, q.device, k=k, v=v, log_gamma=log_gamma, initial_state=initial_state, cu_seqlens=cu_seqlens)
-    args = (_operand(q), _operand(k), _operand(v), log_gamma.detach().float().contiguous(),
+    args = (_operand(q), _operand(k), _operand(v), _decays(log_gamma),
             dk ** -0.5 if scale is None else float(scale), None if initial_state is None else initial_state.contiguous(),
             None if cu_seqlens is None else cu_seqlens.contiguous(), bool(return_state))
     if wants_grad(q, k, v, initial_state):
@@ -197,29 +217,24 @@ def decay_attention_step(q, k, v, log_gamma, state, slots=None, scale: float | N
         raise ValueError(f"ttc_b200 {name}: state must be float32 [n,{H},{dk},{dv}], got "
                          f"{state.dtype} {tuple(state.shape)}")
     B, n = q.shape[0], state.shape[0]
-    if not state[:1].is_contiguous() or state.data_ptr() % 16 or (n > 1 and (state.stride(0) % 4
-                                                                             or state.stride(0) < H * dk * dv)):
+    slot_stride, *inner = state.stride()
+    size = H * dk * dv
+    if n <= 1:
+        slot_stride = size
+    if (inner != [dk * dv, dv, 1] and not state[:1].is_contiguous()) or slot_stride < size or slot_stride % 4 \
+            or state.data_ptr() % 16:
         raise ValueError(f"ttc_b200 {name}: each state must be contiguous and start on a 16-byte boundary")
     if slots is not None and (slots.dtype != torch.int32 or tuple(slots.shape) != (B,)):
         raise ValueError(f"ttc_b200 {name}: slots must be int32 [{B}], got {slots.dtype} {tuple(slots.shape)}")
     if slots is None and n < B:
         raise ValueError(f"ttc_b200 {name}: {B} rows and {n} states")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
+    if (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad) and torch.is_grad_enabled():
         raise ValueError(f"ttc_b200 {name} records no gradient: call it under torch.no_grad()")
     dev = q.device
     _check_device(name, dev, k=k, v=v, log_gamma=log_gamma, state=state, slots=slots)
-    q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
-    log_gamma = log_gamma.detach().float().contiguous()
-    slots = None if slots is None else slots.contiguous()
-    scale = dk ** -0.5 if scale is None else float(scale)
-
-    def call():
-        o = torch.empty(B, H, dv, device=dev, dtype=q.dtype)
-        launch("ttc_decay_attn_step", dev, _lib.load().ttc_decay_attn_step, _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v),
-               _ptr(log_gamma), scale, _ptr(state), state.stride(0) if n > 1 else H * dk * dv, _ptr(slots), B, n, H, Hk,
-               dk, dv, _DTYPES[q.dtype], _ptr(o))
-        return o
-
-    o = on_device(dev, call)
+    if not (q.stride(-1) == k.stride(-1) == v.stride(-1) == 1):
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    o = on_device(dev, _step, q, k, v, _decays(log_gamma), dk ** -0.5 if scale is None else float(scale), state,
+                  slot_stride, None if slots is None else slots.contiguous(), (B, n, H, Hk, dk, dv, _DTYPES[q.dtype]))
     torch.autograd.graph.increment_version(state)
     return o
