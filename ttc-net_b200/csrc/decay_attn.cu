@@ -215,10 +215,11 @@ struct Plan {
   int seg_len, n_seg, items;
 };
 
-// How a call is split.  One CTA for each (sequence, head, pass) where these fill the GPU; else
-// the sequences are cut into segments of about equal shares of all tokens for two CTAs an SM.  A
-// segment's state costs a second pass over k and v and four trips of its elements through memory, so a
-// segment has at least 512 tokens.
+// How a call is split: one CTA for each (sequence, head, pass), or sequences cut into segments whose states
+// are summed first (a second pass over k and v that takes about 0.6 of the main one's time a block) and joined
+// by a scan.  In units of a block's time on the tcgen05 kernel (1.6 us at 128 x 128): `rounds` of CTAs over the
+// SMs times the blocks of a segment, the sums, and 12 for the two more launches and the states' trips
+// through memory.  The least of it over the number of segments; segments have at least four blocks.
 Plan plan(int64_t T, int n_seq, bool packed, int H, int passes, bool tc) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) != cudaSuccess ||
@@ -228,11 +229,22 @@ Plan plan(int64_t T, int n_seq, bool packed, int H, int passes, bool tc) {
   }
   const int64_t rows = static_cast<int64_t>(n_seq) * H * passes;
   const int64_t slots = (tc ? 1 : 2) * sms;
+  const int64_t blocks = (T + C - 1) / C;
   int64_t len = T;
-  if (rows < slots) {
-    const int64_t all = (packed ? T : T * n_seq) * H * passes;
-    len = std::max<int64_t>(512, (all + slots - 1) / slots);
-    if (!packed && len < T) len = (T + (T + len - 1) / len - 1) / ((T + len - 1) / len);  // segments of one length
+  if (packed) {
+    // the lengths are on the device: equal shares of all tokens, where there are CTAs to spare for them
+    if (2 * rows <= slots) len = std::max<int64_t>(8 * C, (T * H * passes + slots - rows - 1) / (slots - rows));
+  } else if (rows > 0 && rows <= slots) {
+    const auto rounds = [&](int64_t ctas) { return static_cast<double>((ctas + slots - 1) / slots); };
+    double best = static_cast<double>(blocks);
+    for (int64_t n = 2; n <= blocks / 4 && n <= 2 * slots / rows; ++n) {
+      const int64_t each = (blocks + n - 1) / n, used = (blocks + each - 1) / each;
+      const double cost = each * (rounds(rows * used) + 0.6 * rounds(rows * (used - 1))) + 12;
+      if (cost < best) {
+        best = cost;
+        len = each * C;
+      }
+    }
   }
   Plan p;
   p.seg_len = static_cast<int>(std::max<int64_t>(C, (len + C - 1) / C * C));

@@ -13,8 +13,8 @@
 //   warps 0-3    the state: row dv of S^T in DK fp32 registers of its thread, S = gamma^rows S + U
 //                with an ordinary fma (U is summed from zero in TMEM), and S in bf16 to TMEM
 //   warps 4-7    o = f_i O1 + O2, rounded, transposed through shared memory to 16-byte stores
-//   warps 8-11   P = scores times decays, masked, in bf16 to shared memory
-//   warps 12-15  f v in two or three bf16 parts; notes blocks whose v holds Inf or NaN
+//   warps 8-15   f v in two or three bf16 parts; note blocks whose v holds Inf or NaN
+//   warps 8-11   also P = scores times decays, masked, in bf16 to shared memory
 //   warps 16-18  copies of every third block each (three stages): whole blocks by TMA, a sequence's
 //                partial last block by 16-byte asynchronous copies that write zeros for what is not in it
 //   warp 19      issues every tcgen05.mma
@@ -50,7 +50,7 @@ struct TcShape {
 };
 
 struct TcBars {
-  uint64_t full[kTcStages], empty[kTcStages], sc_full, sc_empty, p_full[2], p_empty[2], vs_full, vs_empty, u_full,
+  uint64_t full[kTcStages], empty[kTcStages], sc_full, sc_empty, p_full[2], p_empty[2], vs_full[2], vs_empty[2], u_full,
       u_empty, s_full, s_empty, o_full[2], o_empty[2];
 };
 
@@ -204,8 +204,18 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
   return false;
 }
 
-// The same without waiting.
-__device__ __forceinline__ bool bar_done(uint64_t* bar, uint32_t parity) {
+// For one thread alone; and without waiting.
+__device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, volatile int* gone) {
+  const uint32_t addr = tc::smem_u32(bar);
+#pragma unroll 1
+  for (int n = 0; n < 2000000; ++n) {
+    if (bar_try(addr, parity)) return true;
+    if (*gone != 0) return false;
+  }
+  *gone = 1;
+  return false;
+}
+__device__ __forceinline__ bool one_done(uint64_t* bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
       "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
@@ -213,7 +223,7 @@ __device__ __forceinline__ bool bar_done(uint64_t* bar, uint32_t parity) {
       : "=r"(done)
       : "r"(tc::smem_u32(bar)), "r"(parity)
       : "memory");
-  return __all_sync(0xffffffffu, done);
+  return done != 0;
 }
 
 // Named barrier that tells every thread whether all of them had `ok`.
@@ -315,13 +325,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
     }
     tc::mbar_init(&bars.sc_full, 1);
     tc::mbar_init(&bars.sc_empty, 4);
-    tc::mbar_init(&bars.vs_full, 4);
-    tc::mbar_init(&bars.vs_empty, 1);
     tc::mbar_init(&bars.u_full, 1);
     tc::mbar_init(&bars.u_empty, 4);
     tc::mbar_init(&bars.s_full, 4);
     tc::mbar_init(&bars.s_empty, 1);
     for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&bars.vs_full[i], 4);
+      tc::mbar_init(&bars.vs_empty[i], 1);
       tc::mbar_init(&bars.p_full[i], 4);
       tc::mbar_init(&bars.p_empty[i], 4);
       tc::mbar_init(&bars.o_full[i], 1);
@@ -493,25 +503,64 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
       }
       if (tid == 128) bulk_wait();
     }
-  } else if (warp < 12) {  // ---------------------------------------------------------------- the scores
+  } else if (warp < 16) {  // ------------------------------------------ the decayed values, and the scores
     regs_dec<72>();
-    if (!STATE_ONLY) {
-      // Warp w has rows 16 w .. 16 w + 15 (M = 64: TMEM lanes 32 w ..), a thread rows g and g + 8, columns
-      // 8 n + 2 t + x.  The decay of |i - j| places on the past side (j <= i, or j >= i backwards) is
-      // gamma^(whole groups of 8 between them) times a constant of the thread with 1 to 14 places; in the group that
-      // holds the diagonal it is `own`, 0 beyond it.  No negative powers, whatever gamma.
-      const int w = warp - 8, g = lane >> 2, t = lane & 3, m = lane >> 3, r8 = lane & 7;
-      const uint32_t my = tm + (static_cast<uint32_t>(w * 32) << 16) + S::SC;
-      float edge[2], own[2];
+    // Warps 8-11 take the block's second 32 tokens' values and then its scores, warps 12-15 the first 32's
+    // values: U starts on them one by one, and the tile is held half as long as with one warpgroup.
+    const int h2 = warp < 12 ? 1 : 0, t4 = tid & 127;
+    const uint32_t my_off = swz(t4 >> 3, t4 & 7);  // of row t4 / 8; rows 16 further have the same swizzle
+    // Scores: warp w has rows 16 w .. 16 w + 15 (M = 64: TMEM lanes 32 w ..), a thread rows g and g + 8, columns
+    // 8 n + 2 t + x.  The decay of |i - j| places on the past side (j <= i, or j >= i backwards) is
+    // gamma^(whole groups of 8 between them) times a constant of the thread with 1 to 14 places; in the group that
+    // holds the diagonal it is `own`, 0 beyond it.  No negative powers, whatever gamma.
+    const int w = warp & 3, g = lane >> 2, t = lane & 3, m = lane >> 3, r8 = lane & 7;
+    const uint32_t my = tm + (static_cast<uint32_t>(w * 32) << 16) + S::SC;
+    float edge[2], own[2];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int d = rev ? 2 * t + x - g : g - 2 * t - x;
-        edge[x] = pw[8 + d];
-        own[x] = d >= 0 ? P.a * pw[max(d, 0)] : 0.f;
-      }
-      bool see[2] = {rev ? 2 * t >= g : g >= 2 * t, rev ? 2 * t + 1 >= g : g >= 2 * t + 1};
+    for (int x = 0; x < 2; ++x) {
+      const int d = rev ? 2 * t + x - g : g - 2 * t - x;
+      edge[x] = pw[8 + d];
+      own[x] = d >= 0 ? P.a * pw[max(d, 0)] : 0.f;
+    }
+    bool see[2] = {rev ? 2 * t >= g : g >= 2 * t, rev ? 2 * t + 1 >= g : g >= 2 * t + 1};
 #pragma unroll 1
-      for (int c = 0; c < blocks; ++c) {
+    for (int c = 0; c < blocks; ++c) {
+      const int rows = min(C, seg_rows - c * C), s = c % kTcStages;
+      if (!wait_bar(&bars.full[s], (c / kTcStages) & 1, gone)) break;
+      if (c > 0 && !wait_bar(&bars.vs_empty[h2], (c - 1) & 1, gone)) break;
+      const char* const vt = smem + s * S::STAGE + 2 * S::KB;
+      __nv_bfloat162 chk = __floats2bfloat162_rn(0.f, 0.f);
+      auto scale = [&](auto tag) {
+        constexpr int N = decltype(tag)::value;
+#pragma unroll
+        for (int x = 0; x < DV / 32; ++x) {
+          const int r = h2 * 32 + (x & 1) * 16 + (t4 >> 3);
+          const uint32_t off = (x >> 1) * 8192 + (h2 * 32 + (x & 1) * 16) * 128 + my_off;
+          const uint4 w = *reinterpret_cast<const uint4*>(vt + off);
+          const int at = rev ? C - 1 - r : r;  // place in the block
+          const float f = at < rows ? P.u * pw[max(rows - 1 - at + P.e, 0)] : 0.f;
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+          uint32_t o[4][N];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            chk = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&u[y]), __floats2bfloat162_rn(0.f, 0.f), chk);
+            decayed<N>(u[y], f, o[y]);
+          }
+#pragma unroll
+          for (int p = 0; p < N; ++p)
+            *reinterpret_cast<uint4*>(smem + S::PARTS + p * S::VB + off) = make_uint4(o[0][p], o[1][p], o[2][p], o[3][p]);
+        }
+      };
+      if (parts == 3)
+        scale(std::integral_constant<int, 3>{});
+      else
+        scale(std::integral_constant<int, 2>{});
+      if (__low2float(chk) != 0.f || __high2float(chk) != 0.f)  // NaN too
+        *static_cast<volatile int*>(&bad_s[s]) = c + 1;
+      tc::fence_smem_to_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.vs_full[h2]);
+      if (!STATE_ONLY && h2) {
         const int b = c & 1;
         if (c > 1 && !wait_bar(&bars.p_empty[b], ((c >> 1) - 1) & 1, gone)) break;
         if (!wait_bar(&bars.sc_full, c & 1, gone)) break;
@@ -556,50 +605,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
         if (lane == 0) mbar_arrive(&bars.p_full[b]);
       }
     }
-  } else if (warp < 16) {  // ----------------------------------------------------- the decayed values
-    regs_dec<64>();
-    const int t4 = tid - 384;
-    const uint32_t my_off = swz(t4 >> 3, t4 & 7);  // of row t4 / 8; rows 16 further have the same swizzle
-#pragma unroll 1
-    for (int c = 0; c < blocks; ++c) {
-      const int rows = min(C, seg_rows - c * C), s = c % kTcStages;
-      if (!wait_bar(&bars.full[s], (c / kTcStages) & 1, gone)) break;
-      if (c > 0 && !wait_bar(&bars.vs_empty, (c - 1) & 1, gone)) break;
-      const char* const vt = smem + s * S::STAGE + 2 * S::KB;
-      __nv_bfloat162 chk = __floats2bfloat162_rn(0.f, 0.f);
-      auto scale = [&](auto tag) {
-        constexpr int N = decltype(tag)::value;
-#pragma unroll 2
-        for (int x = 0; x < C * DV / 8 / 128; ++x) {
-          const int r = ((x * 16) & 63) + (t4 >> 3);
-          const uint32_t off = (x >> 2) * 8192 + ((x & 3) * 16) * 128 + my_off;
-          const uint4 w = *reinterpret_cast<const uint4*>(vt + off);
-          const int at = rev ? C - 1 - r : r;  // place in the block
-          const float f = at < rows ? P.u * pw[max(rows - 1 - at + P.e, 0)] : 0.f;
-          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-          uint32_t o[4][N];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            chk = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&u[y]), __floats2bfloat162_rn(0.f, 0.f), chk);
-            decayed<N>(u[y], f, o[y]);
-          }
-#pragma unroll
-          for (int p = 0; p < N; ++p)
-            *reinterpret_cast<uint4*>(smem + S::PARTS + p * S::VB + off) = make_uint4(o[0][p], o[1][p], o[2][p], o[3][p]);
-        }
-      };
-      if (parts == 3)
-        scale(std::integral_constant<int, 3>{});
-      else
-        scale(std::integral_constant<int, 2>{});
-      if (__low2float(chk) != 0.f || __high2float(chk) != 0.f)  // NaN too
-        *static_cast<volatile int*>(&bad_s[s]) = c + 1;
-      tc::fence_smem_to_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.vs_full);
-    }
   } else {
-    regs_dec<56>();
+    regs_dec<48>();
     if (warp < 16 + kTcStages) {  // ------------------------------------------------------- the copies
       const int s = warp - 16;
       const uint32_t base = tc::smem_u32(smem) + s * S::STAGE;
@@ -654,25 +661,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
       }
       // no copy is left in flight, whatever made the roles leave
       if (last >= 0) tc::mbar_wait(&bars.full[s], (last / kTcStages) & 1, 0, 10000);
-    } else {  // ----------------------------------------------------------------------- the MMAs
+    } else if (tc::elect_one()) {  // --------------------------------- the MMAs, all from one thread
       const uint32_t base = desc_lo(tc::smem_u32(smem));  // descriptors count in units of 16 bytes
       const int kd16 = (P.kd + 15) / 16;
       constexpr uint32_t d_sc = idesc_bf16(64, 64, false, false), d_u = idesc_bf16(128, DK, true, true),
                          d_o1 = idesc_bf16(128, 64, false, false), d_o2 = idesc_bf16(128, 64, true, false);
       auto scores = [&](int c) {
         const uint32_t q = base + (c % kTcStages) * (S::STAGE / 16), k = q + S::KB / 16;
-        if (!wait_bar(&bars.full[c % kTcStages], (c / kTcStages) & 1, gone)) return false;
-        if (c > 0 && !wait_bar(&bars.sc_empty, (c - 1) & 1, gone)) return false;
+        if (!wait_one(&bars.full[c % kTcStages], (c / kTcStages) & 1, gone)) return false;
+        if (c > 0 && !wait_one(&bars.sc_empty, (c - 1) & 1, gone)) return false;
         tc::fence_after_sync();
-        if (tc::elect_one()) {
-#pragma unroll 2
-          for (int x = 0; x < kd16; ++x) {
-            const uint32_t off = (x >> 2) * 512 + (x & 3) * 2;
-            mma_ss(tm + S::SC, q + off, k + off, d_sc, x > 0);
-          }
-          tc::mma_commit(&bars.sc_full);
+#pragma unroll
+        for (int x = 0; x < DK / 16; ++x) {
+          const uint32_t off = (x >> 2) * 512 + (x & 3) * 2;
+          if (x < kd16) mma_ss(tm + S::SC, q + off, k + off, d_sc, x > 0);
         }
-        __syncwarp();
+        tc::mma_commit(&bars.sc_full);
         return true;
       };
       bool ok = STATE_ONLY || blocks == 0 || scores(0);
@@ -680,50 +684,46 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
       for (int c = 0; ok && c < blocks; ++c) {
         const int s = c % kTcStages, b = c & 1;
         const uint32_t q = base + s * (S::STAGE / 16), k = q + S::KB / 16, v = k + S::KB / 16;
-        if (!(ok = wait_bar(&bars.vs_full, c & 1, gone))) break;
-        if (c + 1 < blocks || keep_last) {
-          if (c > 0 && !(ok = wait_bar(&bars.u_empty, (c - 1) & 1, gone))) break;
+        const bool update = c + 1 < blocks || keep_last;
+        for (int h2 = 0; ok && h2 < 2; ++h2) {  // the tokens' halves, as the decayed values come
+          ok = wait_one(&bars.vs_full[h2], c & 1, gone);
+          if (!update || !ok) continue;
+          if (h2 == 0 && c > 0 && !(ok = wait_one(&bars.u_empty, (c - 1) & 1, gone))) break;
           tc::fence_after_sync();
-          if (tc::elect_one()) {
-            // the small parts first
+          uint32_t a = base + (S::PARTS + (parts - 1) * S::VB) / 16 + h2 * 256;
+          // the small parts first
 #pragma unroll 1
-            for (int p = parts - 1; p >= 0; --p)
-#pragma unroll 2
-              for (int x = 0; x < C / 16; ++x)
-                mma_ss(tm + S::U, base + (S::PARTS + p * S::VB) / 16 + x * 128, k + x * 128, d_u, p < parts - 1 || x > 0);
-            tc::mma_commit(&bars.vs_empty);
-            tc::mma_commit(&bars.u_full);
+          for (int p = parts - 1; p >= 0; --p, a -= S::VB / 16) {
+            mma_ss(tm + S::U, a, k + h2 * 256, d_u, p < parts - 1 || h2 > 0);
+            mma_ss(tm + S::U, a + 128, k + h2 * 256 + 128, d_u, 1);
           }
-          __syncwarp();
+          tc::mma_commit(&bars.vs_empty[h2]);
+          if (h2) tc::mma_commit(&bars.u_full);
         }
+        if (!ok) break;
         if (STATE_ONLY) continue;
-        if (!(ok = wait_bar(&bars.s_full, c & 1, gone))) break;
-        if (c > 1 && !(ok = wait_bar(&bars.o_empty[b], ((c >> 1) - 1) & 1, gone))) break;
+        if (!(ok = wait_one(&bars.s_full, c & 1, gone))) break;
+        if (c > 1 && !(ok = wait_one(&bars.o_empty[b], ((c >> 1) - 1) & 1, gone))) break;
         tc::fence_after_sync();
-        if (tc::elect_one()) {
-#pragma unroll 2
-          for (int x = 0; x < kd16; ++x)
-            mma_ts(tm + S::O + 128 * b, tm + S::S + x * 8, q + (x >> 2) * 512 + (x & 3) * 2, d_o1, x > 0);
-          tc::mma_commit(&bars.s_empty);
-        }
-        __syncwarp();
+#pragma unroll
+        for (int x = 0; x < DK / 16; ++x)
+          if (x < kd16) mma_ts(tm + S::O + 128 * b, tm + S::S + x * 8, q + (x >> 2) * 512 + (x & 3) * 2, d_o1, x > 0);
+        tc::mma_commit(&bars.s_empty);
         // this block's last product next if its scores are there, the next block's scores if only its data is
-        const bool early = c + 1 < blocks && !bar_done(&bars.p_full[b], (c >> 1) & 1) &&
-                           bar_done(&bars.full[(c + 1) % kTcStages], ((c + 1) / kTcStages) & 1);
+        const bool early = c + 1 < blocks && !one_done(&bars.p_full[b], (c >> 1) & 1) &&
+                           one_done(&bars.full[(c + 1) % kTcStages], ((c + 1) / kTcStages) & 1);
         if (early && !(ok = scores(c + 1))) break;
-        if (!(ok = wait_bar(&bars.p_full[b], (c >> 1) & 1, gone))) break;
+        if (!(ok = wait_one(&bars.p_full[b], (c >> 1) & 1, gone))) break;
         tc::fence_after_sync();
-        if (tc::elect_one()) {
-          const uint32_t p = base + S::p_off(parts) / 16 + b * (S::PB / 16);
-#pragma unroll 2
-          for (int x = 0; x < C / 16; ++x) mma_ss(tm + S::O + 128 * b + 64, v + x * 128, p + x * 2, d_o2, x > 0);
-          tc::mma_commit(&bars.o_full[b]);
-        }
-        __syncwarp();
+        const uint32_t p = base + S::p_off(parts) / 16 + b * (S::PB / 16);
+#pragma unroll
+        for (int x = 0; x < C / 16; ++x) mma_ss(tm + S::O + 128 * b + 64, v + x * 128, p + x * 2, d_o2, x > 0);
+        tc::mma_commit(&bars.o_full[b]);
         if (!early && c + 1 < blocks && !(ok = scores(c + 1))) break;
       }
     }
   }
+  __syncwarp();
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();

@@ -89,7 +89,7 @@ int launch_tc_shape(const Args& A, int passes, int* status, cudaStream_t st) {
   const int smem = TcShape<DK, DV>::smem(A.parts);
   TcMaps M{};
   if (int rc = make_maps(A, passes, M)) return rc;
-  // the warpgroups' register shares (192 + 96 + 72 + 64 + 56) are taken from what the CTA is launched with
+  // the warpgroups' register shares (192 + 96 + 72 + 72 + 48) are taken from what the CTA is launched with
   cudaFuncAttributes at;
   cudaError_t e = cudaFuncGetAttributes(&at, k);
   if (e == cudaSuccess && at.numRegs < 96)
