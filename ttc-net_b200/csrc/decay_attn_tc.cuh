@@ -3,7 +3,7 @@
 //
 // Products of a block (M = 128 TMEM lanes, dv of them used, rows are independent; M = 64 for the scores):
 //   Sc [i x j]   = q k^T                A = q, B = k                  (shared memory, K-major)
-//   U  [dv x dk] = (f v)^T k            A = f v in bf16 parts, B = k  (shared memory, MN-major)
+//   U  [dv x dk] = (f v)^T k            A = (f v)^T in bf16 parts in TMEM, B = k (shared memory, MN-major)
 //   O1 [dv x i]  = bf16(S)^T q^T        A = S^T in TMEM, B = q        (K-major)
 //   O2 [dv x i]  = v^T P^T              A = v (MN-major), B = P       (K-major)
 // One shared-memory image of a tile serves as K-major and as MN-major operand: halves of 64 columns, rows of
@@ -13,11 +13,14 @@
 //   warps 0-3    the state: row dv of S^T in DK fp32 registers of its thread, S = gamma^rows S + U
 //                with an ordinary fma (U is summed from zero in TMEM), and S in bf16 to TMEM
 //   warps 4-7    o = f_i O1 + O2, rounded, transposed through shared memory to 16-byte stores
-//   warps 8-15   f v in two or three bf16 parts; note blocks whose v holds Inf or NaN
+//   warps 8-15   (f v)^T in two or three bf16 parts to TMEM; note blocks whose v holds Inf or NaN
 //   warps 8-11   also P = scores times decays, masked, in bf16 to shared memory
-//   warps 16-18  copies of every third block each (three stages): whole blocks by TMA, a sequence's
-//                partial last block by 16-byte asynchronous copies that write zeros for what is not in it
-//   warp 19      issues every tcgen05.mma
+//   warp 16      copies, four to six blocks ahead: whole blocks by TMA, a sequence's partial last block by
+//                16-byte asynchronous copies that write zeros for what is not in it
+//   warps 18, 19 issue the tcgen05.mma's: scores and outputs, and U (one thread for all was the longest chain)
+// What bounds it at 128 x 128 is shared memory: 208 KB of reads and writes a block, 1 600 cycles of its 128 bytes a
+// cycle (272 KB with the parts of f v in shared memory too), then the chain load - parts - U and scores - O2 a
+// stage is held for.
 // Rows of a block lie in token order; in a backward pass the later row is the earlier place.
 // Every wait is bounded (wait_bar); one that runs out makes all roles leave and sets
 // TTC_STATUS_MMA_TIMEOUT in the status word.
@@ -34,24 +37,25 @@
 namespace ttc {
 namespace da {
 
-constexpr int kTcThreads = 640, kTcStages = 3;
+constexpr int kTcThreads = 640;
 
 template <int DK, int DV>
 struct TcShape {
   static constexpr int KB = C * DK * 2, VB = C * DV * 2;
   static constexpr int STAGE = 2 * KB + VB;  // q, k, v
+  static constexpr int STAGES = DK + DV <= 128 ? 6 : 4;
   static constexpr int PB = C * C * 2;
-  static constexpr int PARTS = kTcStages * STAGE;  // f v, part by part
-  __host__ __device__ static constexpr int p_off(int parts) { return PARTS + parts * VB; }
-  __host__ __device__ static constexpr int o_off(int parts) { return p_off(parts) + 2 * PB; }
-  static constexpr int smem(int parts) { return 1024 + o_off(parts) + VB; }
-  // TMEM columns
-  static constexpr int U = 0, S = 128, SC = 192, O = 256;  // O: two buffers of (O1 64, O2 64)
+  static constexpr int P_OFF = STAGES * STAGE;  // two blocks' P
+  static constexpr int O_OFF = P_OFF + 2 * PB;  // a block's outputs on their way
+  static constexpr int SMEM = 1024 + O_OFF + VB;
+  // TMEM columns: U, bf16(S), scores, O1 and O2, the parts of f v
+  static constexpr int U = 0, S = 128, SC = 192, O = 256, F = 384;
 };
 
+template <int STAGES>
 struct TcBars {
-  uint64_t full[kTcStages], empty[kTcStages], sc_full, sc_empty, p_full[2], p_empty[2], vs_full[2], vs_empty[2], u_full,
-      u_empty, s_full, s_empty, o_full[2], o_empty[2];
+  uint64_t full[STAGES], empty[STAGES], noted[STAGES], sc_full, sc_empty, p_full[2], p_empty[2], vs_full[2], vs_empty[2], u_full, u_empty,
+      s_full, s_empty, o_full, o_empty;
 };
 
 // Tensor maps [batch, head, token, dim], boxes of 64 tokens x 64 dims, 128-byte swizzle: a pass reads q, k, v
@@ -159,14 +163,14 @@ __device__ __forceinline__ void tma_out(const CUtensorMap* map, uint32_t src, in
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-// PARTS bf16 parts of f times the two bf16 values in u (no care for Inf: such blocks are noted anyway).
+// PARTS bf16 parts of (f, h) times the two bf16 values in u (no care for Inf: such blocks are noted anyway).
 template <int PARTS>
-__device__ __forceinline__ void decayed(uint32_t u, float f, uint32_t (&o)[PARTS]) {
+__device__ __forceinline__ void decayed(uint32_t u, float f, float h, uint32_t (&o)[PARTS]) {
   float x, y;
-  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %4};\n\tmul.rn.f32x2 p, p, q;\n\t"
+  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmul.rn.f32x2 p, p, q;\n\t"
       "mov.b64 {%0, %1}, p;\n\t}"
       : "=f"(x), "=f"(y)
-      : "f"(mma::lo_f(u)), "f"(mma::hi_f(u)), "f"(f));
+      : "f"(mma::lo_f(u)), "f"(mma::hi_f(u)), "f"(f), "f"(h));
 #pragma unroll
   for (int p = 0; p < PARTS; ++p) {
     o[p] = mma::pack2(x, y);
@@ -176,6 +180,11 @@ __device__ __forceinline__ void decayed(uint32_t u, float f, uint32_t (&o)[PARTS
           : "+f"(x), "+f"(y)
           : "f"(mma::lo_f(o[p])), "f"(mma::hi_f(o[p])));
   }
+}
+// 16 lanes x 8 columns from ldmatrix's registers: a, b the lanes 0-7 and 8-15 of columns 0-3, c, d of 4-7.
+__device__ __forceinline__ void tmem_st_frag(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(bar)) : "memory");
@@ -204,7 +213,7 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
   return false;
 }
 
-// For one thread alone; and without waiting.
+// For one thread alone.
 __device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, volatile int* gone) {
   const uint32_t addr = tc::smem_u32(bar);
 #pragma unroll 1
@@ -215,17 +224,6 @@ __device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, volatil
   *gone = 1;
   return false;
 }
-__device__ __forceinline__ bool one_done(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(tc::smem_u32(bar)), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-
 // Named barrier that tells every thread whether all of them had `ok`.
 __device__ __forceinline__ bool sync_all(int id, int count, bool ok) {
   uint32_t all;
@@ -287,9 +285,10 @@ template <int DK, int DV, bool STATE_ONLY>
 __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __grid_constant__ Args A, const __grid_constant__ TcMaps M, int* status) {
   using S = TcShape<DK, DV>;
   extern __shared__ char smem_raw[];
-  __shared__ TcBars bars;
+  constexpr int STAGES = S::STAGES;
+  __shared__ TcBars<STAGES> bars;
   __shared__ uint32_t tmem_base;
-  __shared__ int gone_s, bad_s[kTcStages];
+  __shared__ int gone_s, bad_s[STAGES];
   __shared__ float pw[72];
   char* const smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
   const Pass& P = A.pass[blockIdx.z];
@@ -318,9 +317,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
 
   volatile int* const gone = &gone_s;
   if (tid == 0) {
-    for (int i = 0; i < kTcStages; ++i) {
+    for (int i = 0; i < STAGES; ++i) {
       tc::mbar_init(&bars.full[i], 1);
       tc::mbar_init(&bars.empty[i], STATE_ONLY ? 4 : 8);
+      tc::mbar_init(&bars.noted[i], 8);
       bad_s[i] = 0;
     }
     tc::mbar_init(&bars.sc_full, 1);
@@ -334,9 +334,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
       tc::mbar_init(&bars.vs_empty[i], 1);
       tc::mbar_init(&bars.p_full[i], 4);
       tc::mbar_init(&bars.p_empty[i], 4);
-      tc::mbar_init(&bars.o_full[i], 1);
-      tc::mbar_init(&bars.o_empty[i], 4);
     }
+    tc::mbar_init(&bars.o_full, 1);
+    tc::mbar_init(&bars.o_empty, 4);
     gone_s = 0;
     tc::mbar_init_fence();
   }
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&bars.u_empty);
-          mbar_arrive(&bars.empty[c % kTcStages]);
+          mbar_arrive(&bars.empty[c % STAGES]);
         }
       }
     }
@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
     if (!STATE_ONLY) {
       const int w4 = warp - 4, g = lane >> 2, t = lane & 3, m = lane >> 3, r8 = lane & 7, v0 = w4 * 32;
       const uint32_t my = tm + (static_cast<uint32_t>(w4 * 32) << 16) + S::O;
-      const uint32_t ot = tc::smem_u32(smem) + S::o_off(parts);
+      const uint32_t ot = tc::smem_u32(smem) + S::O_OFF;
       const int64_t row = static_cast<int64_t>(A.H) * P.vd;  // elements between a head's tokens
       int64_t at = (bi * A.T + first) * row + h * static_cast<int64_t>(P.vd);  // the block's first row
       float f[8][2];  // of rows 8 n + 2 t (+ 1)
@@ -431,16 +431,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
         }
 #pragma unroll 1
       for (int c = 0; c < blocks; ++c, at += down * row) {
-        const int rows = min(C, seg_rows - c * C), s = c % kTcStages, b = c & 1;
+        const int rows = min(C, seg_rows - c * C), s = c % STAGES, b = c & 1;
         const int lo = rev ? C - rows : 0, hi = lo + rows;  // the block's rows that are in the sequence
-        bool ok = wait_bar(&bars.o_full[b], (c >> 1) & 1, gone);
+        bool ok = wait_bar(&bars.o_full, c & 1, gone);
+        // both halves' notes on Inf and NaN; by stage, since those warps may be several blocks ahead
+        ok = ok && wait_bar(&bars.noted[s], (c / STAGES) & 1, gone);
         if (tid == 128) bulk_wait_read();  // the staging has left
         // all four warps go on or none
         if (!sync_all(1, 128, ok)) break;
         tc::fence_after_sync();
         const bool bad = *static_cast<volatile int*>(&bad_s[s]) == c + 1;
         if (bad)
-          outputs_by_term(P, my + 128 * b, smem + S::p_off(parts) + b * S::PB, smem + s * S::STAGE + 2 * S::KB, pw, v0, lo,
+          outputs_by_term(P, my, smem + S::P_OFF + b * S::PB, smem + s * S::STAGE + 2 * S::KB, pw, v0, lo,
                           hi, at, row);
         __syncwarp();
         if (lane == 0) {
@@ -453,8 +455,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
             const int vh = v0 + 16 * hl;
             if (vh < P.vd) {
               float o1[32], o2[32];
-              tmem_ld_frag(my + (16u << 16) * hl + 128 * b, o1);
-              tmem_ld_frag(my + (16u << 16) * hl + 128 * b + 64, o2);
+              tmem_ld_frag(my + (16u << 16) * hl, o1);
+              tmem_ld_frag(my + (16u << 16) * hl + 64, o2);
               tmem_wait_ld(o1, o2);
 #pragma unroll
               for (int q = 0; q < 32; q += 2) fma2(o1[q], o1[q + 1], f[q >> 2][0], f[q >> 2][1], o2[q], o2[q + 1]);
@@ -478,7 +480,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
         }
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.o_empty[b]);
+        if (lane == 0) mbar_arrive(&bars.o_empty);
         if (!P.o_f32 && !bad) {
           tc::fence_smem_to_async();
           tc::named_sync(1, 128);
@@ -496,7 +498,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
               const int i = x / (DV / 8), p8 = x % (DV / 8);
               if (i >= lo && i < hi && p8 * 8 < P.vd)
                 *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(P.o) + at + i * row + p8 * 8) =
-                    *reinterpret_cast<const uint4*>(smem + S::o_off(parts) + (p8 >> 3) * 8192 + swz(i, p8 & 7));
+                    *reinterpret_cast<const uint4*>(smem + S::O_OFF + (p8 >> 3) * 8192 + swz(i, p8 & 7));
             }
           }
         }
@@ -507,14 +509,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
     regs_dec<72>();
     // Warps 8-11 take the block's second 32 tokens' values and then its scores, warps 12-15 the first 32's
     // values: U starts on them one by one, and the tile is held half as long as with one warpgroup.
-    const int h2 = warp < 12 ? 1 : 0, t4 = tid & 127;
-    const uint32_t my_off = swz(t4 >> 3, t4 & 7);  // of row t4 / 8; rows 16 further have the same swizzle
+    // Warp w has value rows (TMEM lanes) 32 w .. 32 w + 31; ldmatrix turns a 16 x 16 corner of v into the layout
+    // of a 16-lane TMEM store, two tokens a register: thread (g, t) has tokens 2t, 2t + 1 (+ 8) of rows g (+ 8).
+    const int h2 = warp < 12 ? 1 : 0;
     // Scores: warp w has rows 16 w .. 16 w + 15 (M = 64: TMEM lanes 32 w ..), a thread rows g and g + 8, columns
     // 8 n + 2 t + x.  The decay of |i - j| places on the past side (j <= i, or j >= i backwards) is
     // gamma^(whole groups of 8 between them) times a constant of the thread with 1 to 14 places; in the group that
     // holds the diagonal it is `own`, 0 beyond it.  No negative powers, whatever gamma.
     const int w = warp & 3, g = lane >> 2, t = lane & 3, m = lane >> 3, r8 = lane & 7;
-    const uint32_t my = tm + (static_cast<uint32_t>(w * 32) << 16) + S::SC;
+    const uint32_t lanes = tm + (static_cast<uint32_t>(w * 32) << 16), my = lanes + S::SC;
     float edge[2], own[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -525,47 +528,60 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
     bool see[2] = {rev ? 2 * t >= g : g >= 2 * t, rev ? 2 * t + 1 >= g : g >= 2 * t + 1};
 #pragma unroll 1
     for (int c = 0; c < blocks; ++c) {
-      const int rows = min(C, seg_rows - c * C), s = c % kTcStages;
-      if (!wait_bar(&bars.full[s], (c / kTcStages) & 1, gone)) break;
+      const int rows = min(C, seg_rows - c * C), s = c % STAGES;
+      if (!wait_bar(&bars.full[s], (c / STAGES) & 1, gone)) break;
       if (c > 0 && !wait_bar(&bars.vs_empty[h2], (c - 1) & 1, gone)) break;
-      const char* const vt = smem + s * S::STAGE + 2 * S::KB;
+      tc::fence_after_sync();
+      const uint32_t vt = tc::smem_u32(smem) + s * S::STAGE + 2 * S::KB;
       __nv_bfloat162 chk = __floats2bfloat162_rn(0.f, 0.f);
-      auto scale = [&](auto tag) {
+      auto decay = [&](auto tag) {
         constexpr int N = decltype(tag)::value;
 #pragma unroll
-        for (int x = 0; x < DV / 32; ++x) {
-          const int r = h2 * 32 + (x & 1) * 16 + (t4 >> 3);
-          const uint32_t off = (x >> 1) * 8192 + (h2 * 32 + (x & 1) * 16) * 128 + my_off;
-          const uint4 w = *reinterpret_cast<const uint4*>(vt + off);
-          const int at = rev ? C - 1 - r : r;  // place in the block
-          const float f = at < rows ? P.u * pw[max(rows - 1 - at + P.e, 0)] : 0.f;
-          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-          uint32_t o[4][N];
+        for (int x = 0; x < 2; ++x) {  // 16 tokens each
+          float f[2][2];  // of tokens 2t (+ 1), + 8
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            chk = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&u[y]), __floats2bfloat162_rn(0.f, 0.f), chk);
-            decayed<N>(u[y], f, o[y]);
+            const int j = h2 * 32 + x * 16 + (y >> 1) * 8 + 2 * t + (y & 1), at = rev ? C - 1 - j : j;
+            f[y >> 1][y & 1] = at < rows ? P.u * pw[max(rows - 1 - at + P.e, 0)] : 0.f;
           }
 #pragma unroll
-          for (int p = 0; p < N; ++p)
-            *reinterpret_cast<uint4*>(smem + S::PARTS + p * S::VB + off) = make_uint4(o[0][p], o[1][p], o[2][p], o[3][p]);
+          for (int z = 0; z < 2; ++z) {  // 16 value rows each
+            const int col = w * 32 + z * 16;
+            uint32_t u[4], o[4][N];
+            mma::ldsm4t(u, vt + (col >> 6) * 8192 + swz(h2 * 32 + x * 16 + (m >> 1) * 8 + r8, ((col & 63) >> 3) + (m & 1)));
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              chk = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&u[y]), __floats2bfloat162_rn(0.f, 0.f), chk);
+              decayed<N>(u[y], f[y >> 1][0], f[y >> 1][1], o[y]);
+            }
+#pragma unroll
+            for (int p = 0; p < N; ++p)
+              tmem_st_frag(lanes + (static_cast<uint32_t>(z * 16) << 16) + S::F + 32 * p + h2 * 16 + x * 8, o[0][p], o[1][p],
+                           o[2][p], o[3][p]);
+          }
         }
       };
-      if (parts == 3)
-        scale(std::integral_constant<int, 3>{});
-      else
-        scale(std::integral_constant<int, 2>{});
-      if (__low2float(chk) != 0.f || __high2float(chk) != 0.f)  // NaN too
-        *static_cast<volatile int*>(&bad_s[s]) = c + 1;
-      tc::fence_smem_to_async();
+      if (w * 32 < DV) {
+        if (parts == 3)
+          decay(std::integral_constant<int, 3>{});
+        else
+          decay(std::integral_constant<int, 2>{});
+        if (__low2float(chk) != 0.f || __high2float(chk) != 0.f)  // NaN too
+          *static_cast<volatile int*>(&bad_s[s]) = c + 1;
+        tc::tmem_wait_st();
+      }
+      tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.vs_full[h2]);
+      if (lane == 0) {
+        mbar_arrive(&bars.vs_full[h2]);
+        if (!STATE_ONLY) mbar_arrive(&bars.noted[s]);
+      }
       if (!STATE_ONLY && h2) {
         const int b = c & 1;
         if (c > 1 && !wait_bar(&bars.p_empty[b], ((c >> 1) - 1) & 1, gone)) break;
         if (!wait_bar(&bars.sc_full, c & 1, gone)) break;
         tc::fence_after_sync();
-        const uint32_t pt = tc::smem_u32(smem) + S::p_off(parts) + b * S::PB;
+        const uint32_t pt = tc::smem_u32(smem) + S::P_OFF + b * S::PB;
         float v[8], next[8];
         tmem_ld_frag(my, next);
 #pragma unroll 1
@@ -607,9 +623,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
     }
   } else {
     regs_dec<48>();
-    if (warp < 16 + kTcStages) {  // ------------------------------------------------------- the copies
-      const int s = warp - 16;
-      const uint32_t base = tc::smem_u32(smem) + s * S::STAGE;
+    if (warp == 16) {  // ------------------------------------------------------- the copies
       const CUtensorMap* const maps[3] = {&M.map[M.m[blockIdx.z][0]], &M.map[M.m[blockIdx.z][1]],
                                           &M.map[M.m[blockIdx.z][2]]};
       const int hq = h / P.qg, hk = h / P.kg, hv = h / P.vg;
@@ -625,13 +639,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
             mma::cp16(dst + hf * 8192 + swz(r, lane & 7), on ? src + ((row + r) * strides[1] + x) * 2 : src, on ? 16 : 0);
           }
       };
-      int last = -1;
+      int sent = 0;
 #pragma unroll 1
-      for (int c = s; c < blocks; c += kTcStages) {
-        const int rows = min(C, seg_rows - c * C);
-        if (c >= kTcStages && !wait_bar(&bars.empty[s], ((c / kTcStages) - 1) & 1, gone)) break;
+      for (int c = 0; c < blocks; ++c) {
+        const int rows = min(C, seg_rows - c * C), s = c % STAGES;
+        if (c >= STAGES && !wait_bar(&bars.empty[s], ((c / STAGES) - 1) & 1, gone)) break;
         const int64_t row = first + down * c;
-        last = c;
+        const uint32_t base = tc::smem_u32(smem) + s * S::STAGE;
+        sent = c + 1;
         if (rows == C) {
           if (tc::elect_one()) {
             constexpr int BOXES = (STATE_ONLY ? 1 : 2) * (DK / 64) + DV / 64;
@@ -660,15 +675,41 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
         }
       }
       // no copy is left in flight, whatever made the roles leave
-      if (last >= 0) tc::mbar_wait(&bars.full[s], (last / kTcStages) & 1, 0, 10000);
-    } else if (tc::elect_one()) {  // --------------------------------- the MMAs, all from one thread
+      for (int c = max(0, sent - STAGES); c < sent; ++c) tc::mbar_wait(&bars.full[c % STAGES], (c / STAGES) & 1, 0, 10000);
+    } else if (warp == 19 && tc::elect_one()) {  // -------------------- the sums U, from one thread
       const uint32_t base = desc_lo(tc::smem_u32(smem));  // descriptors count in units of 16 bytes
+      constexpr uint32_t d_u = idesc_bf16(128, DK, false, true);
+      bool ok = true;
+#pragma unroll 1
+      for (int c = 0; ok && (c + 1 < blocks || (keep_last && c < blocks)); ++c) {
+        const uint32_t k = base + ((c % STAGES) * S::STAGE + S::KB) / 16;
+        if (c > 0 && !(ok = wait_one(&bars.u_empty, (c - 1) & 1, gone))) break;
+#pragma unroll
+        for (int h2 = 0; h2 < 2; ++h2) {  // the tokens' halves, as the decayed values come
+          if (!(ok = ok && wait_one(&bars.vs_full[h2], c & 1, gone))) break;
+          tc::fence_after_sync();
+          const uint32_t a = tm + S::F + h2 * 16, b = k + h2 * 256;
+          // the small parts first
+          if (parts == 3) {
+            mma_ts(tm + S::U, a + 64, b, d_u, h2 > 0);
+            mma_ts(tm + S::U, a + 72, b + 128, d_u, 1);
+          }
+          mma_ts(tm + S::U, a + 32, b, d_u, parts == 3 || h2 > 0);
+          mma_ts(tm + S::U, a + 40, b + 128, d_u, 1);
+          mma_ts(tm + S::U, a, b, d_u, 1);
+          mma_ts(tm + S::U, a + 8, b + 128, d_u, 1);
+          tc::mma_commit(&bars.vs_empty[h2]);
+          if (h2) tc::mma_commit(&bars.u_full);
+        }
+      }
+    } else if (!STATE_ONLY && warp == 18 && tc::elect_one()) {  // ----- the scores and outputs, from another
+      const uint32_t base = desc_lo(tc::smem_u32(smem));
       const int kd16 = (P.kd + 15) / 16;
-      constexpr uint32_t d_sc = idesc_bf16(64, 64, false, false), d_u = idesc_bf16(128, DK, true, true),
-                         d_o1 = idesc_bf16(128, 64, false, false), d_o2 = idesc_bf16(128, 64, true, false);
+      constexpr uint32_t d_sc = idesc_bf16(64, 64, false, false), d_o1 = idesc_bf16(128, 64, false, false),
+                         d_o2 = idesc_bf16(128, 64, true, false);
       auto scores = [&](int c) {
-        const uint32_t q = base + (c % kTcStages) * (S::STAGE / 16), k = q + S::KB / 16;
-        if (!wait_one(&bars.full[c % kTcStages], (c / kTcStages) & 1, gone)) return false;
+        const uint32_t q = base + (c % STAGES) * (S::STAGE / 16), k = q + S::KB / 16;
+        if (!wait_one(&bars.full[c % STAGES], (c / STAGES) & 1, gone)) return false;
         if (c > 0 && !wait_one(&bars.sc_empty, (c - 1) & 1, gone)) return false;
         tc::fence_after_sync();
 #pragma unroll
@@ -679,47 +720,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
         tc::mma_commit(&bars.sc_full);
         return true;
       };
-      bool ok = STATE_ONLY || blocks == 0 || scores(0);
+      bool ok = blocks == 0 || scores(0);
 #pragma unroll 1
       for (int c = 0; ok && c < blocks; ++c) {
-        const int s = c % kTcStages, b = c & 1;
-        const uint32_t q = base + s * (S::STAGE / 16), k = q + S::KB / 16, v = k + S::KB / 16;
-        const bool update = c + 1 < blocks || keep_last;
-        for (int h2 = 0; ok && h2 < 2; ++h2) {  // the tokens' halves, as the decayed values come
-          ok = wait_one(&bars.vs_full[h2], c & 1, gone);
-          if (!update || !ok) continue;
-          if (h2 == 0 && c > 0 && !(ok = wait_one(&bars.u_empty, (c - 1) & 1, gone))) break;
-          tc::fence_after_sync();
-          uint32_t a = base + (S::PARTS + (parts - 1) * S::VB) / 16 + h2 * 256;
-          // the small parts first
-#pragma unroll 1
-          for (int p = parts - 1; p >= 0; --p, a -= S::VB / 16) {
-            mma_ss(tm + S::U, a, k + h2 * 256, d_u, p < parts - 1 || h2 > 0);
-            mma_ss(tm + S::U, a + 128, k + h2 * 256 + 128, d_u, 1);
-          }
-          tc::mma_commit(&bars.vs_empty[h2]);
-          if (h2) tc::mma_commit(&bars.u_full);
-        }
-        if (!ok) break;
-        if (STATE_ONLY) continue;
+        const int b = c & 1;
+        const uint32_t q = base + (c % STAGES) * (S::STAGE / 16), v = q + 2 * S::KB / 16;
         if (!(ok = wait_one(&bars.s_full, c & 1, gone))) break;
-        if (c > 1 && !(ok = wait_one(&bars.o_empty[b], ((c >> 1) - 1) & 1, gone))) break;
+        if (c > 0 && !(ok = wait_one(&bars.o_empty, (c - 1) & 1, gone))) break;
         tc::fence_after_sync();
 #pragma unroll
         for (int x = 0; x < DK / 16; ++x)
-          if (x < kd16) mma_ts(tm + S::O + 128 * b, tm + S::S + x * 8, q + (x >> 2) * 512 + (x & 3) * 2, d_o1, x > 0);
+          if (x < kd16) mma_ts(tm + S::O, tm + S::S + x * 8, q + (x >> 2) * 512 + (x & 3) * 2, d_o1, x > 0);
         tc::mma_commit(&bars.s_empty);
-        // this block's last product next if its scores are there, the next block's scores if only its data is
-        const bool early = c + 1 < blocks && !one_done(&bars.p_full[b], (c >> 1) & 1) &&
-                           one_done(&bars.full[(c + 1) % kTcStages], ((c + 1) / kTcStages) & 1);
-        if (early && !(ok = scores(c + 1))) break;
         if (!(ok = wait_one(&bars.p_full[b], (c >> 1) & 1, gone))) break;
         tc::fence_after_sync();
-        const uint32_t p = base + S::p_off(parts) / 16 + b * (S::PB / 16);
+        const uint32_t p = base + (S::P_OFF + b * S::PB) / 16;
 #pragma unroll
-        for (int x = 0; x < C / 16; ++x) mma_ss(tm + S::O + 128 * b + 64, v + x * 128, p + x * 2, d_o2, x > 0);
-        tc::mma_commit(&bars.o_full[b]);
-        if (!early && c + 1 < blocks && !(ok = scores(c + 1))) break;
+        for (int x = 0; x < C / 16; ++x) mma_ss(tm + S::O + 64, v + x * 128, p + x * 2, d_o2, x > 0);
+        tc::mma_commit(&bars.o_full);
+        if (c + 1 < blocks && !(ok = scores(c + 1))) break;
       }
     }
   }

@@ -86,7 +86,7 @@ int make_maps(const Args& A, int passes, TcMaps& M) {
 template <int DK, int DV, bool STATE_ONLY>
 int launch_tc_shape(const Args& A, int passes, int* status, cudaStream_t st) {
   auto k = decay_attn_tc_kernel<DK, DV, STATE_ONLY>;
-  const int smem = TcShape<DK, DV>::smem(A.parts);
+  constexpr int smem = TcShape<DK, DV>::SMEM;
   TcMaps M{};
   if (int rc = make_maps(A, passes, M)) return rc;
   // the warpgroups' register shares (192 + 96 + 72 + 72 + 48) are taken from what the CTA is launched with
