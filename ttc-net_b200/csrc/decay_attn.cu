@@ -208,19 +208,16 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// bf16 heads run on tcgen05 (decay_attn_tc.cuh) from this width on.
-bool use_tc(int dtype, int dk, int dv) { return dtype == TTC_DTYPE_BF16 && std::max(dk, dv) > 32; }
-
 struct Plan {
   int seg_len, n_seg, items;
 };
 
 // How a call is split: one CTA for each (sequence, head, pass), or sequences cut into segments whose states
-// are summed first (a second pass over k and v that takes about 0.6 of the main one's time a block) and joined
-// by a scan.  In units of a block's time on the tcgen05 kernel (1.6 us at 128 x 128): `rounds` of CTAs over the
-// SMs times the blocks of a segment, the sums, and 12 for the two more launches and the states' trips
-// through memory.  The least of it over the number of segments; segments have at least four blocks.
-Plan plan(int64_t T, int n_seq, bool packed, int H, int passes, bool tc) {
+// are summed first (a second pass over k and v) and joined by a scan.  In units of a block's time on one CTA
+// (1.6 us in bf16, 9 us in fp32 at 64 x 64): `rounds` of CTAs over the SMs times the blocks of a segment, 0.6 of that
+// for the sums (0.4 in fp32), and 12 (2) for the two more launches and the states' trips through memory.  The least
+// of it over the number of segments; segments have at least four blocks.
+Plan plan(int64_t T, int n_seq, bool packed, int H, int passes, int dtype) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
@@ -228,7 +225,7 @@ Plan plan(int64_t T, int n_seq, bool packed, int H, int passes, bool tc) {
     sms = 148;
   }
   const int64_t rows = static_cast<int64_t>(n_seq) * H * passes;
-  const int64_t slots = (tc ? 1 : 2) * sms;
+  const int64_t slots = sms;
   const int64_t blocks = (T + C - 1) / C;
   int64_t len = T;
   if (packed) {
@@ -239,7 +236,8 @@ Plan plan(int64_t T, int n_seq, bool packed, int H, int passes, bool tc) {
     double best = static_cast<double>(blocks);
     for (int64_t n = 2; n <= blocks / 4 && n <= 2 * slots / rows; ++n) {
       const int64_t each = (blocks + n - 1) / n, used = (blocks + each - 1) / each;
-      const double cost = each * (rounds(rows * used) + 0.6 * rounds(rows * (used - 1))) + 12;
+      const double sums = dtype == TTC_DTYPE_BF16 ? 0.6 : 0.4, more = dtype == TTC_DTYPE_BF16 ? 12 : 2;
+      const double cost = each * (rounds(rows * used) + sums * rounds(rows * (used - 1))) + more;
       if (cost < best) {
         best = cost;
         len = each * C;
@@ -284,13 +282,13 @@ int64_t state_bytes(const Plan& p, int64_t T, int H, int dk, int dv, int passes)
   return segmented(p, T) ? static_cast<int64_t>(p.items) * H * dk * dv * 4 * passes : 0;
 }
 
-int run_passes(Args& A, const Pass* pass, int n, int dtype, bool seg, bool tc, int* status, cudaStream_t st) {
+int run_passes(Args& A, const Pass* pass, int n, int dtype, bool seg, int* status, cudaStream_t st) {
   const auto go = [&](const Args& a, int m, bool state_only) {
-    return dtype == TTC_DTYPE_BF16 ? launch_bf16(a, m, state_only, tc, status, st) : launch_f32(a, m, state_only, st);
+    return dtype == TTC_DTYPE_BF16 ? launch_bf16(a, m, state_only, status, st) : launch_f32(a, m, state_only, st);
   };
-  const auto same = [tc](const Pass& x, const Pass& y) {
-    if (tc) return (x.kd > 64) == (y.kd > 64) && (x.vd > 64) == (y.vd > 64);
-    return width_class(x.kd) == width_class(y.kd) && width_class(x.vd) == width_class(y.vd);
+  const auto width = dtype == TTC_DTYPE_BF16 ? width_class_bf16 : width_class_f32;
+  const auto same = [&](const Pass& x, const Pass& y) {
+    return width(x.kd) == width(y.kd) && width(x.vd) == width(y.vd);
   };
   for (int phase = seg ? 0 : 2; phase < 3; ++phase) {
     if (phase == 1) {
@@ -326,7 +324,7 @@ extern "C" int64_t ttc_decay_attn_workspace(int64_t T, int n_seq, int packed, in
   if (int rc = da::check(T, n_seq, H, Hk, dk, dv, dtype)) return -rc;
   if (n_seq == 0) return 0;
   const int passes = backward ? 3 : 1;
-  int64_t bytes = da::state_bytes(da::plan(T, n_seq, packed != 0, H, passes, da::use_tc(dtype, dk, dv)), T, H, dk, dv, passes);
+  int64_t bytes = da::state_bytes(da::plan(T, n_seq, packed != 0, H, passes, dtype), T, H, dk, dv, passes);
   if (backward && H != Hk) bytes += 2 * (packed ? 1 : n_seq) * T * H * dk * 4;
   return bytes;
 }
@@ -343,7 +341,7 @@ extern "C" int ttc_decay_attn_fwd(const void* q, const void* k, const void* v, c
   const void* ops[3] = {q, k, v};
   for (int i = 0; i < 3; ++i)
     if (int rc = da::check_operand(ops[i], strides + 3 * i, 3, dtype)) return rc;
-  const da::Plan p = da::plan(T, n_seq, cu_seqlens != nullptr, H, 1, da::use_tc(dtype, dk, dv));
+  const da::Plan p = da::plan(T, n_seq, cu_seqlens != nullptr, H, 1, dtype);
   const int64_t need = da::state_bytes(p, T, H, dk, dv, 1);
   if (workspace_bytes < need || (need > 0 && (!workspace || da::misaligned16(workspace))))
     return da::fail(TTC_ERR_INVALID, "decay_attn_fwd: workspace missing, misaligned or smaller than ttc_decay_attn_workspace");
@@ -368,7 +366,7 @@ extern "C" int ttc_decay_attn_fwd(const void* q, const void* k, const void* v, c
   f.seg = da::segmented(p, T) ? static_cast<float*>(workspace) : nullptr;
   f.kd = dk, f.vd = dv;
   f.a = f.b = scale, f.u = 1.f;
-  return da::run_passes(A, &f, 1, dtype, f.seg != nullptr, da::use_tc(dtype, dk, dv), status,
+  return da::run_passes(A, &f, 1, dtype, f.seg != nullptr, status,
                         static_cast<cudaStream_t>(stream));
 }
 
@@ -386,7 +384,7 @@ extern "C" int ttc_decay_attn_bwd(const void* q, const void* k, const void* v, c
     if (int rc = da::check_operand(ops[i], strides + 3 * i, 3, dtype)) return rc;
   const int64_t gs[3] = {T * H * dv, static_cast<int64_t>(H) * dv, dv};
   if (int rc = da::check_operand(g_o, gs, 0, dtype)) return rc;
-  const da::Plan p = da::plan(T, n_seq, cu_seqlens != nullptr, H, 3, da::use_tc(dtype, dk, dv));
+  const da::Plan p = da::plan(T, n_seq, cu_seqlens != nullptr, H, 3, dtype);
   const int64_t sbytes = da::state_bytes(p, T, H, dk, dv, 3);
   const int grp = H / Hk;
   const int64_t rows = (cu_seqlens ? 1 : n_seq) * T;
@@ -438,7 +436,7 @@ extern "C" int ttc_decay_attn_bwd(const void* q, const void* k, const void* v, c
   dkp.init = g_final_state, dkp.isk = 1, dkp.isv = dv;
   dkp.kd = dv, dkp.vd = dk, dkp.b = 1.f, dkp.u = scale, dkp.e = 1, dkp.reverse = 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int rc = da::run_passes(A, ps, 3, dtype, ps[0].seg != nullptr, da::use_tc(dtype, dk, dv), status, st)) return rc;
+  if (int rc = da::run_passes(A, ps, 3, dtype, ps[0].seg != nullptr, status, st)) return rc;
   if (grp == 1 || rows == 0) return TTC_OK;
   const int64_t n4 = rows * Hk * dk / 4;
   const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((n4 + 255) / 256, 148 * 16));

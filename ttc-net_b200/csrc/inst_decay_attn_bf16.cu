@@ -106,8 +106,7 @@ int launch_tc_shape(const Args& A, int passes, int* status, cudaStream_t st) {
   return set_error(TTC_ERR_CUDA, buf);
 }
 
-int launch_bf16(const Args& A, int passes, bool state_only, bool tc, int* status, cudaStream_t st) {
-  if (!tc) return launch<1>(A, passes, state_only, st);
+int launch_bf16(const Args& A, int passes, bool state_only, int* status, cudaStream_t st) {
   const bool wide_k = A.pass[0].kd > 64, wide_v = A.pass[0].vd > 64;
 #define TTC_TC(K, V)                                                                   \
   return state_only ? launch_tc_shape<K, V, true>(A, passes, status, st) : launch_tc_shape<K, V, false>(A, passes, status, st)
