@@ -15,8 +15,8 @@
 //   warps 4-7    o = f_i O1 + O2, rounded, transposed through shared memory to 16-byte stores
 //   warps 8-15   (f v)^T in two or three bf16 parts to TMEM; note blocks whose v holds Inf or NaN
 //   warps 8-11   also P = scores times decays, masked, in bf16 to shared memory
-//   warp 16      copies, four to six blocks ahead: whole blocks by TMA, a sequence's partial last block by
-//                16-byte asynchronous copies that write zeros for what is not in it
+//   warp 16      copies by TMA, four to six blocks ahead; zeros in what a sequence's partial last block
+//                holds of others
 //   warps 18, 19 issue the tcgen05.mma's: scores and outputs, and U (one thread for all was the longest chain)
 // What bounds it at 128 x 128 is shared memory: 208 KB of reads and writes a block, 1 600 cycles of its 128 bytes a
 // cycle (272 KB with the parts of f v in shared memory too), then the chain load - parts - U and scores - O2 a
@@ -54,7 +54,7 @@ struct TcShape {
 
 template <int STAGES>
 struct TcBars {
-  uint64_t full[STAGES], empty[STAGES], noted[STAGES], sc_full, sc_empty, p_full[2], p_empty[2], vs_full[2], vs_empty[2], u_full, u_empty,
+  uint64_t full[STAGES], empty[STAGES], noted[STAGES], part, sc_full, sc_empty, p_full[2], p_empty[2], vs_full[2], vs_empty[2], u_full, u_empty,
       s_full, s_empty, o_full, o_empty;
 };
 
@@ -323,6 +323,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
       tc::mbar_init(&bars.noted[i], 8);
       bad_s[i] = 0;
     }
+    tc::mbar_init(&bars.part, 1);
     tc::mbar_init(&bars.sc_full, 1);
     tc::mbar_init(&bars.sc_empty, 4);
     tc::mbar_init(&bars.u_full, 1);
@@ -627,18 +628,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
       const CUtensorMap* const maps[3] = {&M.map[M.m[blockIdx.z][0]], &M.map[M.m[blockIdx.z][1]],
                                           &M.map[M.m[blockIdx.z][2]]};
       const int hq = h / P.qg, hk = h / P.kg, hv = h / P.vg;
-      // a partial block: rows lane / 8, + 4, ..; 8 lanes copy a row's 128 bytes of one half
-      auto tile = [&](uint32_t dst, const void* t, const int64_t* strides, int head, int halves, int d, int64_t row,
-                      int lo, int hi) {
-        const char* src = static_cast<const char*>(t) + (bi * strides[0] + head * strides[2]) * 2;
-        for (int hf = 0; hf < halves; ++hf)
-#pragma unroll 1
-          for (int r = lane >> 3; r < C; r += 4) {
-            const int x = hf * 64 + (lane & 7) * 8;
-            const bool on = r >= lo && r < hi && x < d;
-            mma::cp16(dst + hf * 8192 + swz(r, lane & 7), on ? src + ((row + r) * strides[1] + x) * 2 : src, on ? 16 : 0);
-          }
-      };
       int sent = 0;
 #pragma unroll 1
       for (int c = 0; c < blocks; ++c) {
@@ -647,28 +636,34 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
         const int64_t row = first + down * c;
         const uint32_t base = tc::smem_u32(smem) + s * S::STAGE;
         sent = c + 1;
-        if (rows == C) {
-          if (tc::elect_one()) {
-            constexpr int BOXES = (STATE_ONLY ? 1 : 2) * (DK / 64) + DV / 64;
-            mbar_expect(&bars.full[s], BOXES * 8192);
-            const int r = static_cast<int>(row);
+        uint64_t* const bar = rows == C ? &bars.full[s] : &bars.part;
+        if (tc::elect_one()) {
+          constexpr int BOXES = (STATE_ONLY ? 1 : 2) * (DK / 64) + DV / 64;
+          mbar_expect(bar, BOXES * 8192);
+          const int r = static_cast<int>(row);
 #pragma unroll
-            for (int hf = 0; hf < DK / 64; ++hf) {
-              if (!STATE_ONLY) tma_box(base + hf * 8192, maps[0], hf * 64, r, hq, bi, &bars.full[s]);
-              tma_box(base + S::KB + hf * 8192, maps[1], hf * 64, r, hk, bi, &bars.full[s]);
-            }
-#pragma unroll
-            for (int hf = 0; hf < DV / 64; ++hf)
-              tma_box(base + 2 * S::KB + hf * 8192, maps[2], hf * 64, r, hv, bi, &bars.full[s]);
+          for (int hf = 0; hf < DK / 64; ++hf) {
+            if (!STATE_ONLY) tma_box(base + hf * 8192, maps[0], hf * 64, r, hq, bi, bar);
+            tma_box(base + S::KB + hf * 8192, maps[1], hf * 64, r, hk, bi, bar);
           }
-          __syncwarp();
-        } else {
-          const int lo = rev ? C - rows : 0, hi = lo + rows;
-          if (!STATE_ONLY) tile(base, P.q, P.qs, hq, DK / 64, P.kd, row, lo, hi);
-          tile(base + S::KB, P.k, P.ks, hk, DK / 64, P.kd, row, lo, hi);
-          tile(base + 2 * S::KB, P.v, P.vs, hv, DV / 64, P.vd, row, lo, hi);
-          mma::cp_commit();
-          mma::cp_wait<0>();
+#pragma unroll
+          for (int hf = 0; hf < DV / 64; ++hf) tma_box(base + 2 * S::KB + hf * 8192, maps[2], hf * 64, r, hv, bi, bar);
+        }
+        __syncwarp();
+        if (rows != C) {
+          // The last block's rows that are not in the sequence, another one's or none's, become zeros in k and v:
+          // they may hold Inf or NaN.  (Those of q give outputs that are not stored.)
+          if (!tc::mbar_wait(&bars.part, 0, 0, 10000)) {
+            *gone = 1;
+            break;
+          }
+          const int lo = rev ? 0 : rows, n = C - rows;
+          char* const kv = smem + s * S::STAGE + S::KB;
+#pragma unroll 1
+          for (int x = lane; x < n * 8; x += 32)
+#pragma unroll
+            for (int hf = 0; hf < (DK + DV) / 64; ++hf)
+              *reinterpret_cast<uint4*>(kv + hf * 8192 + lo * 128 + x * 16) = make_uint4(0, 0, 0, 0);
           tc::fence_smem_to_async();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars.full[s]);
