@@ -4,9 +4,12 @@
 // is the turn by -angle with the same factor m.
 //
 // The angle is formed and reduced to [-pi, pi] in 64 bits: at position 10^6 one 32-bit rounding of
-// it is 0.03 rad.  A CTA takes a few tokens, computes the cosines and sines of their pairs once
-// into shared memory (256 / half tokens, so that a thread has about one pair) and streams the
-// heads of q and k past them; bound by memory, each value is read and written once.
+// it is 0.03 rad.  A CTA takes a few tokens (256 / half of them, so that a thread has about one pair), computes their
+// cosines and sines once into shared memory and streams the heads of q and k past them.  Bound by memory,
+// each value is read and written once: 335 MB (4 x 4096 tokens, 32 + 8 heads of 128, bf16) take 60 us, 5.5 TB/s or
+// 0.85 of the copy rate; interleaved 68 us, the same bytes in fp32 58 us (half the angles).  What it took against
+// 67, 77 and 60 us of the first form: loads in flight during the sines, several heads loaded before one is stored, and
+// a table that is read without bank conflicts.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -46,52 +49,165 @@ struct Rot {
   int heads;     // of a CTA (of q's and k's together)
 };
 
+// V values as they lie in memory, and as floats.
 template <typename T, int V>
-__device__ __forceinline__ void load(float (&v)[V], const T* p) {
-  if constexpr (V == 1) {
-    v[0] = ldf(p);
-  } else if constexpr (sizeof(T) == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(p);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-  } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+struct Raw;
+template <typename T>
+struct Raw<T, 1> {
+  T x;
+  __device__ __forceinline__ void load(const T* p) { x = *p; }
+  __device__ __forceinline__ void store(T* p) const { *p = x; }
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = ldf(&x); }
+  __device__ __forceinline__ void set(const float (&v)[1]) { stf(&x, v[0]); }
+};
+template <>
+struct Raw<float, 4> {
+  float4 x;
+  __device__ __forceinline__ void load(const float* p) { x = *reinterpret_cast<const float4*>(p); }
+  __device__ __forceinline__ void store(float* p) const { *reinterpret_cast<float4*>(p) = x; }
+  __device__ __forceinline__ void get(float (&v)[4]) const { v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w; }
+  __device__ __forceinline__ void set(const float (&v)[4]) { x = make_float4(v[0], v[1], v[2], v[3]); }
+};
+template <>
+struct Raw<__nv_bfloat16, 8> {
+  uint4 x;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { x = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void store(__nv_bfloat16* p) const { *reinterpret_cast<uint4*>(p) = x; }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       v[2 * i] = __uint_as_float(u[i] << 16);
       v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
     }
   }
-}
-template <typename T, int V>
-__device__ __forceinline__ void store(T* p, const float (&v)[V]) {
-  if constexpr (V == 1) {
-    stf(p, v[0]);
-  } else if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
+  __device__ __forceinline__ void set(const float (&v)[8]) {
     uint32_t u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
       u[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+    x = make_uint4(u[0], u[1], u[2], u[3]);
   }
-}
+};
 
-// Units of a head: `half / V` (pairs of vectors) or, interleaved, `2 half / V` (vectors of V / 2
-// pairs; V = 1 takes a pair as two scalars), then the vectors that are copied.
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const Rot P) {
-  extern __shared__ float2 cs[];  // [tokens][half]
-  __shared__ int64_t offset[kMaxTokens][2];  // of the tokens in q and k
+// A thread's share: one unit of one token, in every `step`-th head.
+template <typename T, int V, int HEADS, bool ONE>
+struct Share {
+  static constexpr int W = V == 1 ? 1 : ONE ? V / 2 : V;  // pairs of a unit
+  int at, ia, ib;  // place in the table of cosines and sines, < 0 for a copied vector; a pair's vectors
+  int64_t off0, off1;   // of the token in q and k
+  int64_t tok;
+  Raw<T, V> a[HEADS], b[HEADS];
+
+  __device__ __forceinline__ const T* src(const Rot& P, int h) const {
+    return h < P.H[0] ? static_cast<const T*>(P.x[0]) + (off0 + h * P.sh[0])
+                      : static_cast<const T*>(P.x[1]) + (off1 + (h - P.H[0]) * P.sh[1]);
+  }
+  __device__ __forceinline__ T* dst(const Rot& P, int h) const {
+    return h < P.H[0] ? static_cast<T*>(P.y[0]) + (tok * P.H[0] + h) * P.D
+                      : static_cast<T*>(P.y[1]) + (tok * P.H[1] + h - P.H[0]) * P.D;
+  }
+  __device__ __forceinline__ void set(const Rot& P, int64_t tok0, int x, int units, int turn) {
+    const int t = x / units, u = x - t * units;
+    tok = tok0 + t;
+    const int64_t n = tok / P.T;
+    off0 = n * P.sb[0] + (tok - n * P.T) * P.st[0];
+    off1 = n * P.sb[1] + (tok - n * P.T) * P.st[1];
+    at = u < turn ? t * turn + u : -1;
+    ib = 0;
+    if (u >= turn) {
+      ia = 2 * P.half + (u - turn) * V;
+    } else if (ONE) {
+      ia = u * V;
+    } else {
+      ia = P.interleaved ? 2 * u : u * V, ib = P.interleaved ? 2 * u + 1 : u * V + P.half;
+    }
+  }
+  // HEADS heads are loaded before the first of them is stored: a store may alias a later load for all that the
+  // compiler knows.
+  __device__ __forceinline__ void load(const Rot& P, int h, int end, int step) {
+#pragma unroll
+    for (int x = 0; x < HEADS; ++x)
+      if (h + x * step < end) {
+        const T* const from = src(P, h + x * step);
+        a[x].load(from + ia);
+        if (!ONE && at >= 0) b[x].load(from + ib);
+      }
+  }
+  __device__ __forceinline__ void turn_store(const Rot& P, const float2* cs, int plane, int h, int end, int step) {
+    float2 w[W];
+    if (at >= 0) {
+      if constexpr (W == 1) {
+        w[0] = cs[at];
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; i += 2) {
+          const float4 c = reinterpret_cast<const float4*>(cs)[i / 2 * plane + at];
+          w[i] = make_float2(c.x, c.y);
+          w[i + 1] = make_float2(c.z, c.w);
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < HEADS; ++x)
+      if (h + x * step < end) {
+        T* const to = dst(P, h + x * step);
+        if (at >= 0) {
+          float p[V];
+          a[x].get(p);
+          if constexpr (!ONE) {
+            float q[V];
+            b[x].get(q);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const float m = p[i], n = q[i];
+              p[i] = fmaf(m, w[i].x, -n * w[i].y);
+              q[i] = fmaf(m, w[i].y, n * w[i].x);
+            }
+            b[x].set(q);
+            b[x].store(to + ib);
+          } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+              const float m = p[2 * i], n = p[2 * i + 1];
+              p[2 * i] = fmaf(m, w[i].x, -n * w[i].y);
+              p[2 * i + 1] = fmaf(m, w[i].y, n * w[i].x);
+            }
+          }
+          a[x].set(p);
+        }
+        a[x].store(to + ia);
+      }
+  }
+};
+
+// Units of a head: `half / V` (pairs of vectors) or, where a vector holds both values of its pairs (ONE: interleaved,
+// V > 1), `2 half / V`, then the vectors that are copied.  The table holds two neighbouring pairs of a unit in 16 bytes,
+// the units' next to each other (`plane` of them), so that a warp's reads meet no bank twice.
+template <typename T, int V, bool ONE>
+__global__ void __launch_bounds__(kThreads, 5) rotary_kernel(const __grid_constant__ Rot P) {
+  constexpr int HEADS = V == 1 || ONE ? 4 : 2;  // two vectors a head, or one
+  extern __shared__ float4 table[];
+  float2* const cs = reinterpret_cast<float2*>(table);
   const int64_t tok0 = static_cast<int64_t>(blockIdx.x) * P.tokens;
-  const int64_t total = P.B * P.T;
-  const int ntok = static_cast<int>(min(static_cast<int64_t>(P.tokens), total - tok0));
+  const int ntok = static_cast<int>(min(static_cast<int64_t>(P.tokens), P.B * P.T - tok0));
+  const int turn = ONE ? 2 * P.half / V : P.half / V, plane = ntok * turn;
+  const int units = turn + (P.D - 2 * P.half) / V;
+  // thread -> (token, unit), groups of such threads share the heads; the first heads' loads are in flight while the
+  // cosines and sines are computed
+  const int work = ntok * units, lanes = min(work, kThreads), step = kThreads / lanes;
+  const int group = threadIdx.x / lanes, h0 = blockIdx.y * P.heads + group;
+  const int end = group < step ? min(static_cast<int>(blockIdx.y + 1) * P.heads, P.H[0] + P.H[1]) : 0;
+  int x = threadIdx.x % lanes;
+  using My = Share<T, V, HEADS, ONE>;
+  My my;
+  my.set(P, tok0, x, units, turn);
+  my.load(P, h0, end, step);
   for (int i = threadIdx.x; i < ntok * P.half; i += kThreads) {
     const int t = i / P.half, p = i - t * P.half;
-    const int64_t tok = tok0 + t, b = tok / P.T, off = b * P.pb + (tok - b * P.T) * P.pt;
+    const int64_t tok = tok0 + t, n = tok / P.T, off = n * P.pb + (tok - n * P.T) * P.pt;
     const double pos = P.pos64 ? static_cast<double>(static_cast<const int64_t*>(P.pos)[off])
                                : static_cast<double>(static_cast<const int*>(P.pos)[off]);
     const double angle = P.sign * pos * P.inv_freq[p];
@@ -101,66 +217,23 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rot P) {
     const float rh = static_cast<float>(r), rl = static_cast<float>(r - static_cast<double>(rh));
     float s, c;
     sincosf(rh, &s, &c);
-    cs[i] = make_float2(P.mag * fmaf(-s, rl, c), P.mag * fmaf(c, rl, s));
-  }
-  if (threadIdx.x < 2 * ntok) {
-    const int t = threadIdx.x >> 1, w = threadIdx.x & 1;
-    const int64_t tok = tok0 + t, b = tok / P.T;
-    offset[t][w] = b * P.sb[w] + (tok - b * P.T) * P.st[w];
+    const int u = p / My::W, y = p - u * My::W;
+    cs[My::W == 1 ? i : (y / 2 * plane + t * turn + u) * 2 + (y & 1)] =
+        make_float2(P.mag * fmaf(-s, rl, c), P.mag * fmaf(c, rl, s));
   }
   __syncthreads();
-  const bool pairs_split = V == 1 || !P.interleaved;  // a and b of a pair in different units' vectors
-  const int turn = pairs_split ? P.half / V : 2 * P.half / V;
-  const int units = turn + (P.D - 2 * P.half) / V;
-  const int h0 = blockIdx.y * P.heads, nh = min(P.heads, P.H[0] + P.H[1] - h0);
-  // thread -> unit and (token, head); the remaining threads of the last round idle
-  const int lanes = min(units, kThreads), step = kThreads / lanes;
-  const int lane = threadIdx.x % lanes, r0 = threadIdx.x / lanes;
-  if (r0 >= step) return;
-  for (int u = lane; u < units; u += lanes) {
-    int t = r0 / nh, h = r0 - t * nh;
-#pragma unroll 4
-    for (int r = r0; r < ntok * nh; r += step) {
-      const int hh = h0 + h, which = hh >= P.H[0], head = which ? hh - P.H[0] : hh;
-      const T* src = static_cast<const T*>(P.x[which]) + offset[t][which] + head * P.sh[which];
-      T* dst = static_cast<T*>(P.y[which]) + ((tok0 + t) * P.H[which] + head) * P.D;
-      if (u >= turn) {
-        const int c = 2 * P.half + (u - turn) * V;
-        float v[V];
-        load<T, V>(v, src + c);
-        store<T, V>(dst + c, v);
-      } else if (pairs_split) {
-        const int ia = P.interleaved ? 2 * u : u * V, ib = P.interleaved ? 2 * u + 1 : u * V + P.half;
-        float a[V], bb[V];
-        load<T, V>(a, src + ia);
-        load<T, V>(bb, src + ib);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float2 w = cs[t * P.half + u * V + i];
-          const float x = a[i], y = bb[i];
-          a[i] = fmaf(x, w.x, -y * w.y);
-          bb[i] = fmaf(x, w.y, y * w.x);
-        }
-        store<T, V>(dst + ia, a);
-        store<T, V>(dst + ib, bb);
-      } else if constexpr (V > 1) {
-        float a[V];
-        load<T, V>(a, src + u * V);
-#pragma unroll
-        for (int i = 0; i < V / 2; ++i) {
-          const float2 w = cs[t * P.half + u * (V / 2) + i];
-          const float x = a[2 * i], y = a[2 * i + 1];
-          a[2 * i] = fmaf(x, w.x, -y * w.y);
-          a[2 * i + 1] = fmaf(x, w.y, y * w.x);
-        }
-        store<T, V>(dst + u * V, a);
-      }
-      h += step;
-      while (h >= nh) {
-        h -= nh;
-        ++t;
-      }
+#pragma unroll 1
+  while (true) {
+#pragma unroll 1
+    for (int h = h0; h < end;) {
+      my.turn_store(P, cs, plane, h, end, step);
+      h += HEADS * step;
+      my.load(P, h, end, step);
     }
+    x += lanes;
+    if (x >= work) break;
+    my.set(P, tok0, x, units, turn);
+    my.load(P, h0, end, step);
   }
 }
 
@@ -185,10 +258,12 @@ int run(Rot P, cudaStream_t st) {
   if (ctas < 296) P.heads = std::max<int64_t>(4, (all * ctas + 295) / 296);
   const dim3 grid(static_cast<unsigned>(ctas), (all + P.heads - 1) / P.heads);
   const size_t smem = static_cast<size_t>(P.tokens) * P.half * sizeof(float2);
-  if (vec)
-    rotary_kernel<T, VT><<<grid, kThreads, smem, st>>>(P);
+  if (vec && P.interleaved)
+    rotary_kernel<T, VT, true><<<grid, kThreads, smem, st>>>(P);
+  else if (vec)
+    rotary_kernel<T, VT, false><<<grid, kThreads, smem, st>>>(P);
   else
-    rotary_kernel<T, 1><<<grid, kThreads, smem, st>>>(P);
+    rotary_kernel<T, 1, false><<<grid, kThreads, smem, st>>>(P);
   const cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) return TTC_OK;
   char buf[256];
