@@ -217,7 +217,7 @@ struct Plan {
 // (1.6 us in bf16, 9 us in fp32 at 64 x 64): `rounds` of CTAs over the SMs times the blocks of a segment, 0.6 of that
 // for the sums (0.4 in fp32), and 12 (2) for the two more launches and the states' trips through memory.  The least
 // of it over the number of segments; segments have at least four blocks.
-Plan plan(int64_t T, int n_seq, bool packed, int H, int passes, int dtype) {
+Plan plan(int64_t T, int n_seq, bool packed, int H, int dk, int dv, int passes, int dtype) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
@@ -225,7 +225,10 @@ Plan plan(int64_t T, int n_seq, bool packed, int H, int passes, int dtype) {
     sms = 148;
   }
   const int64_t rows = static_cast<int64_t>(n_seq) * H * passes;
-  const int64_t slots = sms;
+  // fp32 heads of at most 32 x 32 leave room for two CTAs on an SM (16 x 512 tokens, 32 heads: backward 471 -> 395 us;
+  // at 32 x 64 the halved registers cost more than the second CTA gives, 239 -> 308)
+  const bool two = dtype == TTC_DTYPE_F32 && width_class_f32(dk) + width_class_f32(dv) <= 64;
+  const int64_t slots = two ? 2 * sms : sms;
   const int64_t blocks = (T + C - 1) / C;
   int64_t len = T;
   if (packed) {
@@ -324,7 +327,7 @@ extern "C" int64_t ttc_decay_attn_workspace(int64_t T, int n_seq, int packed, in
   if (int rc = da::check(T, n_seq, H, Hk, dk, dv, dtype)) return -rc;
   if (n_seq == 0) return 0;
   const int passes = backward ? 3 : 1;
-  int64_t bytes = da::state_bytes(da::plan(T, n_seq, packed != 0, H, passes, dtype), T, H, dk, dv, passes);
+  int64_t bytes = da::state_bytes(da::plan(T, n_seq, packed != 0, H, dk, dv, passes, dtype), T, H, dk, dv, passes);
   if (backward && H != Hk) bytes += 2 * (packed ? 1 : n_seq) * T * H * dk * 4;
   return bytes;
 }
@@ -341,7 +344,7 @@ extern "C" int ttc_decay_attn_fwd(const void* q, const void* k, const void* v, c
   const void* ops[3] = {q, k, v};
   for (int i = 0; i < 3; ++i)
     if (int rc = da::check_operand(ops[i], strides + 3 * i, 3, dtype)) return rc;
-  const da::Plan p = da::plan(T, n_seq, cu_seqlens != nullptr, H, 1, dtype);
+  const da::Plan p = da::plan(T, n_seq, cu_seqlens != nullptr, H, dk, dv, 1, dtype);
   const int64_t need = da::state_bytes(p, T, H, dk, dv, 1);
   if (workspace_bytes < need || (need > 0 && (!workspace || da::misaligned16(workspace))))
     return da::fail(TTC_ERR_INVALID, "decay_attn_fwd: workspace missing, misaligned or smaller than ttc_decay_attn_workspace");
@@ -384,7 +387,7 @@ extern "C" int ttc_decay_attn_bwd(const void* q, const void* k, const void* v, c
     if (int rc = da::check_operand(ops[i], strides + 3 * i, 3, dtype)) return rc;
   const int64_t gs[3] = {T * H * dv, static_cast<int64_t>(H) * dv, dv};
   if (int rc = da::check_operand(g_o, gs, 0, dtype)) return rc;
-  const da::Plan p = da::plan(T, n_seq, cu_seqlens != nullptr, H, 3, dtype);
+  const da::Plan p = da::plan(T, n_seq, cu_seqlens != nullptr, H, dk, dv, 3, dtype);
   const int64_t sbytes = da::state_bytes(p, T, H, dk, dv, 3);
   const int grp = H / Hk;
   const int64_t rows = (cu_seqlens ? 1 : n_seq) * T;

@@ -100,7 +100,7 @@ __device__ __noinline__ void slow_pv(float (&out)[NT][4], const char* Ps, const 
 
 // STATE_ONLY: the sums u gamma^.. k^T v of the segments alone, from a zero state.
 template <int DK, int DV, bool STATE_ONLY>
-__global__ void __launch_bounds__(kF32Threads) decay_attn_f32_kernel(const __grid_constant__ Args A) {
+__global__ void __launch_bounds__(kF32Threads, (DK + DV <= 64 ? 2 : 1)) decay_attn_f32_kernel(const __grid_constant__ Args A) {
   using S = F32Shape<DK, DV, STATE_ONLY>;
   extern __shared__ __align__(128) char smem[];
   const Pass& P = A.pass[blockIdx.z];
