@@ -53,7 +53,7 @@ struct Args {
   int64_t T;      // tokens of a sequence, or of the packed row
   int n_seq, H, seg_len, n_seg;
   int items;  // upper bound on the number of (sequence, segment) pairs
-  int parts;  // bf16 parts of the decayed values in the state update (NP = 1)
+  int parts;  // bf16 only: parts of the decayed values in the state update
 };
 
 struct Item {
