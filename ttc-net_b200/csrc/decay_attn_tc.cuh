@@ -373,31 +373,48 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
         sv = P.isv;
       }
     }
+    // The initial state comes as a first sum U: 32 values a turn of a rolled loop through TMEM, then the blocks' own
+    // update with a factor of 0.  (128 loads in a row took 5 us of a CTA's time, with or without a state, for fetching
+    // their code.)
     float st[DK];
 #pragma unroll
-    for (int k = 0; k < DK; ++k) st[k] = src != nullptr && k < P.kd && vr < P.vd ? src[k * sk + vr * sv] : 0.f;
+    for (int k = 0; k < DK; ++k) st[k] = 0.f;
+    if (src != nullptr) {
+      const float* p = src + vr * sv;
 #pragma unroll 1
-    for (int c = 0; c < blocks; ++c) {
-      const int rows = min(C, seg_rows - c * C);
-      if (!STATE_ONLY) {
-        if (c > 0 && !wait_bar(&bars.s_empty, (c - 1) & 1, gone)) break;
-        tc::fence_after_sync();
+      for (int k0 = 0; k0 < DK; k0 += 32) {
+        float u[32];
 #pragma unroll
-        for (int x = 0; x < DK / 64; ++x) {
-          float w[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) w[i] = __uint_as_float(mma::pack2(st[64 * x + 2 * i], st[64 * x + 2 * i + 1]));
-          tc::tmem_st<32>(my + S::S + 32 * x, w);
-        }
-        tc::tmem_wait_st();
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.s_full);
+        for (int i = 0; i < 32; ++i, p += sk) u[i] = k0 + i < P.kd && vr < P.vd ? *p : 0.f;
+        tc::tmem_st<32>(my + S::U + k0, u);
       }
-      if (c + 1 < blocks || keep_last) {
+      tc::tmem_wait_st();
+    }
+#pragma unroll 1
+    for (int c = -1; c < blocks; ++c) {
+      float keep = 0.f;
+      if (c >= 0) {
+        if (!STATE_ONLY) {
+          if (c > 0 && !wait_bar(&bars.s_empty, (c - 1) & 1, gone)) break;
+          tc::fence_after_sync();
+#pragma unroll
+          for (int x = 0; x < DK / 64; ++x) {
+            float w[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) w[i] = __uint_as_float(mma::pack2(st[64 * x + 2 * i], st[64 * x + 2 * i + 1]));
+            tc::tmem_st<32>(my + S::S + 32 * x, w);
+          }
+          tc::tmem_wait_st();
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.s_full);
+        }
+        if (c + 1 == blocks && !keep_last) break;
         if (!wait_bar(&bars.u_full, c & 1, gone)) break;
         tc::fence_after_sync();
-        const float keep = pw[rows];
+        keep = pw[min(C, seg_rows - c * C)];
+      }
+      if (c >= 0 || src != nullptr) {
 #pragma unroll
         for (int x = 0; x < DK / 32; ++x) {
           float u[32];
@@ -405,12 +422,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
 #pragma unroll
           for (int i = 0; i < 32; i += 2) fma2(st[32 * x + i], st[32 * x + i + 1], keep, keep, u[i], u[i + 1]);
         }
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bars.u_empty);
-          mbar_arrive(&bars.empty[c % STAGES]);
-        }
+      }
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&bars.u_empty);
+        if (c >= 0) mbar_arrive(&bars.empty[c % STAGES]);
       }
     }
     float* dst = nullptr;
@@ -419,9 +436,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
     else if (keep_last)
       dst = P.fin + sbase;
     if (dst != nullptr && vr < P.vd) {
+      float* p = dst + vr;
 #pragma unroll
-      for (int k = 0; k < DK; ++k)
-        if (k < P.kd) dst[static_cast<int64_t>(k) * P.vd + vr] = st[k];
+      for (int k = 0; k < DK; ++k, p += P.vd)
+        if (k < P.kd) *p = st[k];
     }
   } else if (warp < 8) {  // ------------------------------------------------------------ the outputs
     if (!STATE_ONLY) {
@@ -686,7 +704,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
 #pragma unroll 1
       for (int c = 0; ok && (c + 1 < blocks || (keep_last && c < blocks)); ++c) {
         const uint32_t k = base + ((c % STAGES) * S::STAGE + S::KB) / 16;
-        if (c > 0 && !(ok = wait_one(&bars.u_empty, (c - 1) & 1, gone))) break;
+        if (!(ok = wait_one(&bars.u_empty, c & 1, gone))) break;
 #pragma unroll
         for (int h2 = 0; h2 < 2; ++h2) {  // the tokens' halves, as the decayed values come
           if (!(ok = ok && wait_one(&bars.vs_full[h2], c & 1, gone))) break;
