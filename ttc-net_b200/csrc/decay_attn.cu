@@ -28,6 +28,7 @@ __global__ void __launch_bounds__(256) segment_scan_kernel(const __grid_constant
   const int e = blockIdx.x * blockDim.x + threadIdx.x;
   // the first item of this sequence: the segments of the ones before it
   __shared__ int64_t s_first, s_len;
+  __shared__ float s_pow[2];  // of a whole segment and of the last one: once a CTA, an exponential in 64 bits is slow
   if (threadIdx.x < 32) {
     int64_t first = 0, row0 = 0, len = A.T;
     if (A.cu == nullptr) {
@@ -45,14 +46,14 @@ __global__ void __launch_bounds__(256) segment_scan_kernel(const __grid_constant
       s_first = first;
       s_len = len;
     }
+    const int64_t last = len - static_cast<int64_t>(segs_of(A, len) - 1) * A.seg_len;
+    if (threadIdx.x < 2) s_pow[threadIdx.x] = decay_pow(A.log_gamma[h], threadIdx.x ? last : A.seg_len);
   }
   __syncthreads();
   if (e >= size) return;
   const int64_t first = s_first, len = s_len;
   const int segs = segs_of(A, len);
   if (first + segs > A.items) return;  // offsets that are not increasing: more segments than were launched
-  const float lg = A.log_gamma[h];
-  const float whole = decay_pow(lg, A.seg_len);
   const int64_t sbase = (static_cast<int64_t>(n) * A.H + h) * size;
   float run = P.init != nullptr ? P.init[sbase + (e / P.vd) * P.isk + (e % P.vd) * P.isv] : 0.f;
   for (int s = 0; s < segs; ++s) {
@@ -60,11 +61,11 @@ __global__ void __launch_bounds__(256) segment_scan_kernel(const __grid_constant
     if (s + 1 < segs) {
       const float u = *p;
       *p = run;
-      run = fmaf(whole, run, u);
+      run = fmaf(s_pow[0], run, u);
     } else {
       const float u = P.fin != nullptr ? *p : 0.f;
       *p = run;
-      if (P.fin != nullptr) P.fin[sbase + e] = fmaf(decay_pow(lg, len - static_cast<int64_t>(s) * A.seg_len), run, u);
+      if (P.fin != nullptr) P.fin[sbase + e] = fmaf(s_pow[1], run, u);
     }
   }
 }
@@ -214,10 +215,17 @@ struct Plan {
 };
 
 // How a call is split: one CTA for each (sequence, head, pass), or sequences cut into segments whose states
-// are summed first (a second pass over k and v) and joined by a scan.  In units of a block's time on one CTA
-// (1.8 us in bf16 at 128 x 128, 1.4 at 64 x 64; in fp32 7 us at 32 x 64, 9 at 64 x 64): `rounds` of CTAs over the SMs times the blocks of a segment, 0.6 of that
-// for the sums (0.4 in fp32), and 12 (2) for the two more launches and the states' trips through memory.  The least
-// of it over the number of segments; segments have at least four blocks.
+// are summed first (a second pass over k and v) and joined by a scan.  The least cost over the number of segments decides,
+// segments have at least four blocks.  In units of a block's time on one CTA (1.9 us in bf16 at 128 x 128, 1.5 at
+// 64 x 64; in fp32 7 us at 32 x 64, 9 at 64 x 64), `rounds` of CTAs over the SMs cost their segment's blocks and
+// `start` for a CTA's beginning and end; those of the sums `sum` of the blocks and `sum_start`; `more` is for the two
+// further launches, `state` for the trips of one segment's 128 x 128 state through memory.  Fitted to measured times: 8192
+// tokens, 32 heads of 128: 224 us as one, 134 in 4 segments, 187 in 9; 2 x 4096: 116 as one, 129 in 2.
+struct Costs {
+  double start, sum, sum_start, more, state;
+};
+constexpr Costs kCostsBf16 = {3, 0.75, 4, 5, 0.03}, kCostsF32 = {0, 0.4, 0, 2, 0};
+
 Plan plan(int64_t T, int n_seq, bool packed, int H, int dk, int dv, int passes, int dtype) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) != cudaSuccess ||
@@ -237,11 +245,12 @@ Plan plan(int64_t T, int n_seq, bool packed, int H, int dk, int dv, int passes, 
     if (2 * rows <= slots) len = std::max<int64_t>(8 * C, (T * H * passes + slots - rows - 1) / (slots - rows));
   } else if (rows > 0 && rows <= slots) {
     const auto rounds = [&](int64_t ctas) { return static_cast<double>((ctas + slots - 1) / slots); };
-    double best = static_cast<double>(blocks);
+    const Costs c = dtype == TTC_DTYPE_BF16 ? kCostsBf16 : kCostsF32;
+    double best = static_cast<double>(blocks) + c.start;
     for (int64_t n = 2; n <= blocks / 4 && n <= 2 * slots / rows; ++n) {
       const int64_t each = (blocks + n - 1) / n, used = (blocks + each - 1) / each;
-      const double sums = dtype == TTC_DTYPE_BF16 ? 0.6 : 0.4, more = dtype == TTC_DTYPE_BF16 ? 12 : 2;
-      const double cost = each * (rounds(rows * used) + sums * rounds(rows * (used - 1))) + more;
+      const double cost = rounds(rows * used) * (each + c.start) + rounds(rows * (used - 1)) * (c.sum * each + c.sum_start) +
+                          c.more + c.state * static_cast<double>(rows * used) * dk * dv / 16384;
       if (cost < best) {
         best = cost;
         len = each * C;
