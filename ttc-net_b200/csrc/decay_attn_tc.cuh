@@ -25,10 +25,11 @@
 // outputs do behind them (2.3e-3 from the exact outputs in all, 1.7e-3 of it the outputs' own rounding); the state itself
 // stays in fp32, and the decayed values that update it come in two bf16 parts (16 bits, below what an output shows), or
 // three (24 bits) where the last state is asked for (1e-7 to 2e-7 of it).
-// Measured: 8 x 4096 tokens, 32 heads of 128: 238 us (4.5 TB/s), 262 with last states; 4 x 4096, 37 heads (one CTA on
-// each SM) 127 us, 4.9 TB/s; 37 heads of 64: 103 us.  A CTA of one block takes 10 us, of which starting and ending are
-// nine: packed prompts of a few blocks each are bound by that (a form with CTAs that go on with further pieces made
-// every block 7 % slower and was no faster on them).
+// Measured at full clock: 8 x 4096 tokens, 32 heads of 128: 234 us (4.6 TB/s), 258 with last states, 307 in a long run,
+// where the board reaches its power limit; 4 x 4096, 37 heads (one CTA on each SM) 122 us, 5.1 TB/s; 37 heads of 64:
+// 106 us.  A CTA of one block takes 6 us, of which starting and ending are four: packed prompts of a few blocks each
+// are bound by that (a form with CTAs that go on with further pieces made every block 7 % slower and was no faster on
+// them).
 // Rows of a block lie in token order; in a backward pass the later row is the earlier place.
 // Every wait is bounded (wait_bar); one that runs out makes all roles leave and sets
 // TTC_STATUS_MMA_TIMEOUT in the status word.

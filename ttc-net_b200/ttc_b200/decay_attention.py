@@ -111,7 +111,7 @@ def _dims(q, v, cu_seqlens):
 def _forward(q, k, v, log_gamma, scale, initial_state, cu_seqlens, want_state):
     dev, lib, dims = q.device, _lib.load(), _dims(q, v, cu_seqlens)
     T, n_seq, H, _, dk, dv, _ = dims
-    o = torch.empty(v.shape, device=dev, dtype=q.dtype)
+    o = v.new_empty(v.shape)
     state = torch.empty(n_seq, H, dk, dv, device=dev) if want_state else None
     nbytes = lib.ttc_decay_attn_workspace(T, n_seq, cu_seqlens is not None, *dims[2:], 0)
     ws = _workspace(nbytes, dev)
@@ -134,9 +134,8 @@ def _backward(q, k, v, log_gamma, scale, initial_state, cu_seqlens, g_o, g_state
 
 
 def _step(q, k, v, log_gamma, scale, state, slot_stride, slots, dims):
-    dev = q.device
-    o = torch.empty(v.shape, device=dev, dtype=q.dtype)
-    launch("ttc_decay_attn_step", dev, _lib.load().ttc_decay_attn_step, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+    o = v.new_empty(v.shape)
+    launch("ttc_decay_attn_step", q.device, _lib.load().ttc_decay_attn_step, q.data_ptr(), k.data_ptr(), v.data_ptr(),
            _SIX(*_strides(q), *_strides(k), *_strides(v)), log_gamma.data_ptr(), scale, state.data_ptr(), slot_stride,
            _ptr(slots), *dims, o.data_ptr())
     return o
@@ -213,7 +212,7 @@ def decay_attention_step(q, k, v, log_gamma, state, slots=None, scale: float | N
     is outside [0, n) is padding, its output is zeros.  Records no gradient."""
     name = "decay_attention_step"
     H, Hk, dk, dv = _check_qkv(name, q, k, v, log_gamma, 1)
-    if state.dtype != torch.float32 or state.dim() != 4 or tuple(state.shape[1:]) != (H, dk, dv):
+    if state.dtype != torch.float32 or state.dim() != 4 or state.shape[1:] != (H, dk, dv):
         raise ValueError(f"ttc_b200 {name}: state must be float32 [n,{H},{dk},{dv}], got "
                          f"{state.dtype} {tuple(state.shape)}")
     B, n = q.shape[0], state.shape[0]
@@ -224,7 +223,7 @@ def decay_attention_step(q, k, v, log_gamma, state, slots=None, scale: float | N
     if (inner != [dk * dv, dv, 1] and not state[:1].is_contiguous()) or slot_stride < size or slot_stride % 4 \
             or state.data_ptr() % 16:
         raise ValueError(f"ttc_b200 {name}: each state must be contiguous and start on a 16-byte boundary")
-    if slots is not None and (slots.dtype != torch.int32 or tuple(slots.shape) != (B,)):
+    if slots is not None and (slots.dtype != torch.int32 or slots.shape != (B,)):
         raise ValueError(f"ttc_b200 {name}: slots must be int32 [{B}], got {slots.dtype} {tuple(slots.shape)}")
     if slots is None and n < B:
         raise ValueError(f"ttc_b200 {name}: {B} rows and {n} states")
@@ -235,6 +234,6 @@ def decay_attention_step(q, k, v, log_gamma, state, slots=None, scale: float | N
     if not (q.stride(-1) == k.stride(-1) == v.stride(-1) == 1):
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
     o = on_device(dev, _step, q, k, v, _decays(log_gamma), dk ** -0.5 if scale is None else float(scale), state,
-                  slot_stride, None if slots is None else slots.contiguous(), (B, n, H, Hk, dk, dv, _DTYPES[q.dtype]))
+                  slot_stride, slots if slots is None or slots.is_contiguous() else slots.contiguous(), (B, n, H, Hk, dk, dv, _DTYPES[q.dtype]))
     torch.autograd.graph.increment_version(state)
     return o

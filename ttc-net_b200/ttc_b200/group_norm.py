@@ -19,7 +19,7 @@ _ACTS = {"none": _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}
 
 def _rows(t, C):
     """t as [rows, C] with contiguous channels, a view where its strides allow."""
-    t = t.reshape(-1, C)
+    t = t if t.dim() == 2 else t.reshape(-1, C)
     return t if t.stride(1) == 1 or C == 1 else t.contiguous()
 
 
@@ -32,7 +32,7 @@ def _dims(x, weight, bias, groups, act, eps):
 
 def _forward(x, weight, bias, gate, groups, act, eps):
     dims, f32 = _dims(x, weight, bias, groups, act, eps)
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = x.new_empty(x.shape)
     launch("ttc_group_norm_fwd", x.device, _lib.load().ttc_group_norm_fwd, _ptr(x), x.stride(0), _ptr(gate),
            0 if gate is None else gate.stride(0), _ptr(weight), _ptr(bias), f32, *dims, _ptr(y))
     return y
@@ -89,17 +89,18 @@ def group_norm(x, num_groups: int, weight=None, bias=None, gate=None, activation
                          f"{gate.dtype} {tuple(gate.shape)}")
     params = [p for p in (weight, bias) if p is not None]
     for p in params:
-        if tuple(p.shape) != (C,) or p.dtype not in (x.dtype, torch.float32) or p.dtype != params[0].dtype:
+        if p.shape != (C,) or p.dtype not in (x.dtype, torch.float32) or p.dtype != params[0].dtype:
             raise ValueError(f"ttc_b200 group_norm: weight and bias must be [{C}] in {x.dtype} or both float32")
+    dev = x.device
     for t, n in ((weight, "weight"), (bias, "bias"), (gate, "gate")):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"ttc_b200 group_norm: {n} is on {t.device}, x on {x.device}")
+        if t is not None and t.device != dev:
+            raise ValueError(f"ttc_b200 group_norm: {n} is on {t.device}, x on {dev}")
     if not x.is_cuda:
         raise ValueError("ttc_b200 group_norm needs CUDA tensors (there is no CPU path)")
-    args = (_rows(x, C), *(None if p is None else p.contiguous() for p in (weight, bias)),
+    args = (_rows(x, C), *(p if p is None or p.is_contiguous() else p.contiguous() for p in (weight, bias)),
             None if gate is None else _rows(gate, C), int(num_groups), _ACTS[activation], float(eps))
     if wants_grad(x, weight, bias, gate):
         y = GroupNormFunction.apply(*args)
     else:
-        y = on_device(x.device, _forward, *args)
-    return y.view(x.shape)
+        y = on_device(dev, _forward, *args)
+    return y if x.dim() == 2 else y.view(x.shape)

@@ -58,15 +58,16 @@ def _dense(t):
 
 
 def _turn(q, k, positions, inv_freq, interleaved, magnitude, inverse):
-    dev = q.device
     q, k = _dense(q), None if k is None else _dense(k)
-    B, T, H, D = q.shape
-    outs = [None if t is None else torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k)]
-    launch("ttc_rotary", dev, _lib.load().ttc_rotary, _ptr(q), _THREE(*q.stride()[:3]), H, _ptr(k),
-           None if k is None else _THREE(*k.stride()[:3]), 0 if k is None else k.shape[2], _ptr(positions),
-           _TWO(*positions.stride()), positions.dtype == torch.int64, _ptr(inv_freq), B, T, D, inv_freq.numel(),
-           interleaved, inverse, magnitude, _DTYPES[q.dtype], _ptr(outs[0]), _ptr(outs[1]))
-    return outs
+    B, T, H, D = shape = q.shape
+    q_out, k_out = q.new_empty(shape), None if k is None else k.new_empty(k.shape)
+    ps = positions.stride()  # [T] and [1, T] are shared by the batch
+    launch("ttc_rotary", q.device, _lib.load().ttc_rotary, q.data_ptr(), _THREE(*q.stride()[:3]), H, _ptr(k),
+           None if k is None else _THREE(*k.stride()[:3]), 0 if k is None else k.shape[2], positions.data_ptr(),
+           _TWO(0 if len(ps) == 1 or positions.shape[0] == 1 else ps[0], ps[-1]), positions.dtype == torch.int64,
+           inv_freq.data_ptr(), B, T, D, inv_freq.shape[0], interleaved, inverse, magnitude, _DTYPES[q.dtype],
+           q_out.data_ptr(), _ptr(k_out))
+    return q_out, k_out
 
 
 class RotaryFunction(torch.autograd.Function):
@@ -78,7 +79,7 @@ class RotaryFunction(torch.autograd.Function):
         ctx.save_for_backward(positions, inv_freq)
         ctx.how = (interleaved, magnitude)
         ctx.like = tuple(None if t is None else (t.shape, t.dtype, t.device) for t in (q, k))
-        return tuple(on_device(q.device, _turn, q, k, positions, inv_freq, *ctx.how, False))
+        return on_device(q.device, _turn, q, k, positions, inv_freq, *ctx.how, False)
 
     @staticmethod
     @torch.amp.custom_bwd(device_type="cuda")
@@ -112,18 +113,20 @@ def rotary(q, k, positions, inv_freq, interleaved: bool = False, magnitude: floa
         raise ValueError(f"ttc_b200 rotary: q {q.dtype} {tuple(q.shape)} and k {k.dtype} {tuple(k.shape)} do not match")
     if positions.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"ttc_b200 rotary: positions must be int32 or int64, got {positions.dtype}")
-    if tuple(positions.shape) not in ((T,), (1, T), (B, T)):
+    if positions.shape not in ((T,), (1, T), (B, T)):
         raise ValueError(f"ttc_b200 rotary: positions must be [{T}] or [{B},{T}], got {tuple(positions.shape)}")
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or 2 * inv_freq.numel() > D:
         raise ValueError(f"ttc_b200 rotary: inv_freq must be float64 [R / 2] with R <= {D}, got "
                          f"{inv_freq.dtype} {tuple(inv_freq.shape)}")
+    dev = q.device
     for t, n in ((k, "k"), (positions, "positions"), (inv_freq, "inv_freq")):
-        if t is not None and t.device != q.device:
-            raise ValueError(f"ttc_b200 rotary: {n} is on {t.device}, q on {q.device}")
+        if t is not None and t.device != dev:
+            raise ValueError(f"ttc_b200 rotary: {n} is on {t.device}, q on {dev}")
     if not q.is_cuda:
         raise ValueError("ttc_b200 rotary needs CUDA tensors (there is no CPU path)")
-    args = (q, k, positions if positions.shape == (B, T) else positions.expand(B, T), inv_freq.detach().contiguous(),
-            bool(interleaved), float(magnitude))
+    if not inv_freq.is_contiguous():
+        inv_freq = inv_freq.contiguous()
+    args = (q, k, positions, inv_freq, bool(interleaved), float(magnitude))
     if wants_grad(q, k):
-        return RotaryFunction.apply(*args)
-    return tuple(on_device(q.device, _turn, *args, False))
+        return RotaryFunction.apply(q, k, positions, inv_freq.detach(), *args[4:])
+    return on_device(dev, _turn, *args, False)
