@@ -7,6 +7,7 @@ import sys
 
 import pytest
 import torch
+from test_gpu_decay_attention import _check, _inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -179,3 +180,14 @@ def test_a_timeout_is_reported_at_the_next_call():
     with pytest.raises(RuntimeError, match="ran out"):
         ttc_b200.decay_attention(q, k, v, _decays(2))
     assert torch.equal(ttc_b200.decay_attention(q, k, v, _decays(2)), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("lens", [[3] * 50 + [2100] + [70] * 9, [7] * 333])
+def test_many_packed_sequences(lens, dtype):
+    """More sequences than a warp looks at in one turn, one of them cut into segments; and more than there are CTAs."""
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    q, k, v, lg, go, start, gs = _inputs(1, cu[-1] + 2, 1, 1, 32, 64, dtype, n_state=len(lens))
+    _check(q, k, v, lg, go, start, gs, cu=cu)

@@ -92,6 +92,14 @@ __device__ __forceinline__ Item find_item(const Args& A, int x) {
     it.len = A.T;
     return it;
   }
+  if (A.n_seg == 1) {  // no sequence is cut: no search, which would cost a row of many sequences their square
+    it.seq = x < A.n_seq ? x : -1;
+    it.seg = 0;
+    it.index = x;
+    it.row0 = it.len = 0;
+    if (it.seq >= 0) seq_range(A, it.seq, it.row0, it.len);
+    return it;
+  }
   const int lane = threadIdx.x & 31;
   int64_t before = 0;
   for (int n0 = 0; n0 < A.n_seq; n0 += 32) {
