@@ -191,3 +191,22 @@ def test_many_packed_sequences(lens, dtype):
         cu.append(cu[-1] + n)
     q, k, v, lg, go, start, gs = _inputs(1, cu[-1] + 2, 1, 1, 32, 64, dtype, n_state=len(lens))
     _check(q, k, v, lg, go, start, gs, cu=cu)
+
+
+def test_autocast_changes_nothing():
+    """Types are the operands' own, forward and backward, whatever autocast is set around either."""
+    from ttc_b200 import decay_attention, group_norm, rotary, rotary_frequencies
+    f, _ = rotary_frequencies(32)
+    pos, lg = torch.arange(90, device="cuda"), _decays(2)
+    ins = [_normal(i, 2, 90, 2, 32, dtype=torch.float32).requires_grad_() for i in range(3)]
+
+    def call():
+        q, k = rotary(ins[0], ins[1], pos, f)
+        y = group_norm(decay_attention(q, k, ins[2], lg).flatten(2), 2, activation="silu")
+        return [y, *torch.autograd.grad(y, ins, torch.ones_like(y))]
+
+    want = call()
+    with torch.autocast("cuda", torch.bfloat16):
+        got = call()
+    for a, b in zip(got, want):
+        assert a.dtype == torch.float32 and torch.equal(a, b)

@@ -123,7 +123,7 @@ def _forward(q, k, v, log_gamma, scale, initial_state, cu_seqlens, want_state):
 
 def _backward(q, k, v, log_gamma, scale, initial_state, cu_seqlens, g_o, g_state, want_start):
     dev, lib, dims = q.device, _lib.load(), _dims(q, v, cu_seqlens)
-    d_q, d_k, d_v = (torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k, v))
+    d_q, d_k, d_v = (t.new_empty(t.shape) for t in (q, k, v))
     d_s = torch.empty(initial_state.shape, device=dev) if want_start else None
     nbytes = lib.ttc_decay_attn_workspace(*dims[:2], cu_seqlens is not None, *dims[2:], 1)
     ws = _workspace(nbytes, dev)
@@ -145,19 +145,17 @@ class DecayAttentionFunction(torch.autograd.Function):
     """(q, k, v, initial_state) -> (o, last state or None)."""
 
     @staticmethod
-    @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, q, k, v, log_gamma, scale, initial_state, cu_seqlens, want_state):
         ctx.save_for_backward(q, k, v, log_gamma, initial_state, cu_seqlens)
         ctx.scale = scale
         return on_device(q.device, _forward, q, k, v, log_gamma, scale, initial_state, cu_seqlens, want_state)
 
     @staticmethod
-    @torch.amp.custom_bwd(device_type="cuda")
     @once_differentiable
     def backward(ctx, g_o, g_state):
         q, k, v, log_gamma, initial_state, cu_seqlens = ctx.saved_tensors
         g_o = torch.zeros_like(v) if g_o is None else g_o
-        g_o = _aligned(g_o.to(v.dtype).contiguous())
+        g_o = _aligned(g_o.contiguous())
         g_state = None if g_state is None else g_state.float().contiguous()
         want = initial_state is not None and ctx.needs_input_grad[5]
         d_q, d_k, d_v, d_s = on_device(q.device, _backward, q, k, v, log_gamma, ctx.scale, initial_state, cu_seqlens, g_o,

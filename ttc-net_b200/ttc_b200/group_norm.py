@@ -42,7 +42,7 @@ def _backward(x, weight, bias, gate, groups, act, eps, g, needs):
     """(dx, dweight, dbias, dgate), None where not needed."""
     dev, lib = x.device, _lib.load()
     dims, f32 = _dims(x, weight, bias, groups, act, eps)
-    dx, dw, db, dgate = (torch.empty(t.shape, device=dev, dtype=t.dtype) if need and t is not None else None
+    dx, dw, db, dgate = (t.new_empty(t.shape) if need and t is not None else None
                          for need, t in zip(needs, (x, weight, bias, gate)))
     nbytes = lib.ttc_group_norm_workspace(*dims[:3], dims[5]) if dw is not None or db is not None else 0
     ws = _workspace(nbytes, dev)
@@ -56,18 +56,16 @@ class GroupNormFunction(torch.autograd.Function):
     """(x, weight, bias, gate) -> y for x and gate [rows, C], all but x may be None."""
 
     @staticmethod
-    @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, x, weight, bias, gate, groups, act, eps):
         ctx.save_for_backward(x, weight, bias, gate)
         ctx.how = (groups, act, eps)
         return on_device(x.device, _forward, x, weight, bias, gate, groups, act, eps)
 
     @staticmethod
-    @torch.amp.custom_bwd(device_type="cuda")
     @once_differentiable
     def backward(ctx, g):
         saved = ctx.saved_tensors
-        g = g.to(saved[0].dtype).contiguous()
+        g = g.contiguous()
         return (*on_device(g.device, _backward, *saved, *ctx.how, g, ctx.needs_input_grad[:4]), None, None, None)
 
 

@@ -71,28 +71,27 @@ def _turn(q, k, positions, inv_freq, interleaved, magnitude, inverse):
 
 
 class RotaryFunction(torch.autograd.Function):
-    """(q, k or None) -> both turned; the backward turns the gradients back."""
+    """(q, k or None) -> both turned; the backward turns the gradients back.  No autocast wrappers, here as in the other
+    sequence operators: nothing inside depends on its state."""
 
     @staticmethod
-    @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, q, k, positions, inv_freq, interleaved, magnitude):
         ctx.save_for_backward(positions, inv_freq)
         ctx.how = (interleaved, magnitude)
-        ctx.like = tuple(None if t is None else (t.shape, t.dtype, t.device) for t in (q, k))
+        ctx.like = q.shape, None if k is None else k.shape, q.dtype
         return on_device(q.device, _turn, q, k, positions, inv_freq, *ctx.how, False)
 
     @staticmethod
-    @torch.amp.custom_bwd(device_type="cuda")
     @once_differentiable
     def backward(ctx, g_q, g_k):
         positions, inv_freq = ctx.saved_tensors
-        gs = []
-        for g, like in zip((g_q, g_k), ctx.like):
-            if like is not None:
-                shape, dtype, dev = like
-                g = torch.zeros(shape, dtype=dtype, device=dev) if g is None else g.to(dtype)
-            gs.append(g)
-        return (*on_device(gs[0].device, _turn, *gs, positions, inv_freq, *ctx.how, True), None, None, None, None)
+        q_shape, k_shape, dtype = ctx.like
+        if g_q is None:
+            g_q = torch.zeros(q_shape, dtype=dtype, device=positions.device)
+        if g_k is None and k_shape is not None:
+            g_k = torch.zeros(k_shape, dtype=dtype, device=positions.device)
+        d_q, d_k = on_device(positions.device, _turn, g_q, g_k, positions, inv_freq, *ctx.how, True)
+        return d_q, d_k, None, None, None, None
 
 
 def rotary(q, k, positions, inv_freq, interleaved: bool = False, magnitude: float = 1.0):
