@@ -1,6 +1,5 @@
 // Warp-level bf16 matrix products (mma.sync m16n8k16, fp32 accumulators) and what feeds them:
-// ldmatrix / movmatrix, 16-byte asynchronous copies, the swizzled shared-memory tile and the
-// split of an fp32 value into bf16 parts.
+// ldmatrix, the swizzled shared-memory tile and the split of an fp32 value into bf16 parts.
 #pragma once
 
 #include <cuda_bf16.h>
