@@ -4,6 +4,7 @@ the raw handle of the current stream, and autograd's machinery only where a grad
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, solver
 
@@ -25,6 +26,17 @@ def on_device(dev, f, *args):
         return f(*args)
     with torch.cuda.device(dev):
         return f(*args)
+
+
+def refuse_tangents(name, **operands) -> None:
+    """Raises where an operand carries a forward-mode tangent.  The kernels write into new tensors, which
+    have none, and a dual tensor need not require a gradient: the result would pass for a constant."""
+    # the number of the innermost dual level, negative outside of all (a call costs 0.2 us there)
+    if forward_ad._current_level < 0 or not torch._C._is_fwd_grad_enabled():
+        return
+    for n, t in operands.items():
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"ttc_b200 {name} has no forward-mode derivative: {n} carries a tangent")
 
 
 def wants_grad(*tensors) -> bool:

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._call import launch, on_device, wants_grad
+from ._call import launch, on_device, refuse_tangents, wants_grad
 from .solver import _DTYPES, _aligned, _ptr
 
 
@@ -153,6 +153,7 @@ class DecayAttentionFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g_o, g_state):
+        refuse_tangents("decay_attention", g_o=g_o, g_state=g_state)
         q, k, v, log_gamma, initial_state, cu_seqlens = ctx.saved_tensors
         g_o = torch.zeros_like(v) if g_o is None else g_o
         g_o = _aligned(g_o.contiguous())
@@ -168,7 +169,8 @@ def decay_attention(q, k, v, log_gamma, scale: float | None = None, initial_stat
     """o [B, T, H, dv] for q, k [B, T, Hk, dk] and v [B, T, H, dv] (float32 or bfloat16; H a multiple of
     Hk, head h reads key head h // (H // Hk); dk, dv multiples of 8 up to 128), log_gamma [H] the logarithm
     of each head's decay (fixed: no gradient; -inf is no memory).  ``scale`` defaults to
-    dk ** -0.5.  Differentiable in q, k, v and ``initial_state`` [B, H, dk, dv] float32.
+    dk ** -0.5.  Differentiable in q, k, v and ``initial_state`` [B, H, dk, dv] float32, once and
+    in reverse mode.
 
     ``return_state``: (o, state), the states behind the last tokens, float32, from which
     ``decay_attention_step`` or another call goes on.
@@ -192,6 +194,7 @@ def decay_attention(q, k, v, log_gamma, scale: float | None = None, initial_stat
                                       or tuple(initial_state.shape) != (n_seq, H, dk, dv)):
         raise ValueError(f"ttc_b200 {name}: initial_state must be float32 [{n_seq},{H},{dk},{dv}], got "
                          f"{initial_state.dtype} {tuple(initial_state.shape)}")
+    refuse_tangents(name, q=q, k=k, v=v, log_gamma=log_gamma, initial_state=initial_state)
     _check_device(name, q.device, k=k, v=v, log_gamma=log_gamma, initial_state=initial_state, cu_seqlens=cu_seqlens)
     args = (_operand(q), _operand(k), _operand(v), _decays(log_gamma),
             dk ** -0.5 if scale is None else float(scale), None if initial_state is None else initial_state.contiguous(),
@@ -227,6 +230,7 @@ def decay_attention_step(q, k, v, log_gamma, state, slots=None, scale: float | N
         raise ValueError(f"ttc_b200 {name}: {B} rows and {n} states")
     if (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad) and torch.is_grad_enabled():
         raise ValueError(f"ttc_b200 {name} records no gradient: call it under torch.no_grad()")
+    refuse_tangents(name, q=q, k=k, v=v, log_gamma=log_gamma, state=state)
     dev = q.device
     _check_device(name, dev, k=k, v=v, log_gamma=log_gamma, state=state, slots=slots)
     if not (q.stride(-1) == k.stride(-1) == v.stride(-1) == 1):

@@ -10,7 +10,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._call import launch, on_device, wants_grad
+from ._call import launch, on_device, refuse_tangents, wants_grad
 from .decay_attention import _workspace
 from .solver import _DTYPES, _ptr
 
@@ -64,6 +64,7 @@ class GroupNormFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
+        refuse_tangents("group_norm", g=g)
         saved = ctx.saved_tensors
         g = g.contiguous()
         return (*on_device(g.device, _backward, *saved, *ctx.how, g, ctx.needs_input_grad[:4]), None, None, None)
@@ -74,7 +75,8 @@ def group_norm(x, num_groups: int, weight=None, bias=None, gate=None, activation
     at most 1024, each to mean 0 and variance 1 (fp32), times ``weight`` [C] plus ``bias`` [C] (x's dtype
     or float32), then ``activation`` ("none", "silu" or "gelu", the exact one).  With ``gate`` (x's
     shape) the activation is of the gate and multiplies: norm(x) * act(gate).  Rows do not mix, so a
-    token's result does not depend on other tokens.  Differentiable in x, weight, bias and gate."""
+    token's result does not depend on other tokens.  Differentiable in x, weight, bias and gate, once and in
+    reverse mode."""
     if x.dtype not in _DTYPES:
         raise TypeError(f"ttc_b200 group_norm supports float32 and bfloat16, got {x.dtype}")
     if activation not in _ACTS:
@@ -89,6 +91,7 @@ def group_norm(x, num_groups: int, weight=None, bias=None, gate=None, activation
     for p in params:
         if p.shape != (C,) or p.dtype not in (x.dtype, torch.float32) or p.dtype != params[0].dtype:
             raise ValueError(f"ttc_b200 group_norm: weight and bias must be [{C}] in {x.dtype} or both float32")
+    refuse_tangents("group_norm", x=x, weight=weight, bias=bias, gate=gate)
     dev = x.device
     for t, n in ((weight, "weight"), (bias, "bias"), (gate, "gate")):
         if t is not None and t.device != dev:
