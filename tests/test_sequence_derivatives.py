@@ -60,3 +60,27 @@ def test_tangents_of_gradients_are_refused(name, function, grads):
             gs[at] = dual
             with pytest.raises(NotImplementedError, match=f"{name}.*tangent"):
                 backward(None, *gs)
+
+
+FIXED = [("rotary", _rotary, "inv_freq"), ("rotary", _rotary, "magnitude"), ("decay_attention", _attention, "log_gamma"),
+         ("decay_attention", _attention, "scale"), ("decay_attention_step", _step, "log_gamma"),
+         ("decay_attention_step", _step, "scale"), ("group_norm", _norm, "eps")]
+
+
+@pytest.mark.parametrize("name,make,operand", FIXED, ids=[f"{c[0]}-{c[2]}" for c in FIXED])
+def test_what_has_no_gradient_may_not_ask_for_one(name, make, operand):
+    """Decays, frequencies and factors are fixed: a leaf in their place would get no gradient."""
+    import ttc_b200
+    call, args = getattr(ttc_b200, name), make()
+    args[operand] = args.get(operand, torch.tensor(0.5)).clone()
+    with pytest.raises(ValueError, match="CUDA"):
+        call(**args)
+    args[operand].requires_grad_()
+    with pytest.raises(ValueError, match=f"{operand}.* gradient"):
+        call(**args)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        call(**args)
+    with forward_ad.dual_level():
+        args[operand] = forward_ad.make_dual(args[operand].detach(), torch.ones_like(args[operand]))
+        with pytest.raises(NotImplementedError, match="tangent"):
+            call(**args)

@@ -39,5 +39,14 @@ def refuse_tangents(name, **operands) -> None:
             raise NotImplementedError(f"ttc_b200 {name} has no forward-mode derivative: {n} carries a tangent")
 
 
+def refuse_gradient(name, **fixed) -> None:
+    """Raises where one of ``fixed`` (numbers, or tensors in their place) asks for a gradient: there is none."""
+    for n, t in fixed.items():
+        if isinstance(t, torch.Tensor):
+            if t.requires_grad and torch.is_grad_enabled():
+                raise ValueError(f"ttc_b200 {name}: {n} is fixed, it must not require a gradient")
+            refuse_tangents(name, **{n: t})
+
+
 def wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)

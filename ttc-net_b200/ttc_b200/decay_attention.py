@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._call import launch, on_device, refuse_tangents, wants_grad
+from ._call import launch, on_device, refuse_gradient, refuse_tangents, wants_grad
 from .solver import _DTYPES, _aligned, _ptr
 
 
@@ -194,6 +194,7 @@ def decay_attention(q, k, v, log_gamma, scale: float | None = None, initial_stat
                                       or tuple(initial_state.shape) != (n_seq, H, dk, dv)):
         raise ValueError(f"ttc_b200 {name}: initial_state must be float32 [{n_seq},{H},{dk},{dv}], got "
                          f"{initial_state.dtype} {tuple(initial_state.shape)}")
+    refuse_gradient(name, scale=scale)
     refuse_tangents(name, q=q, k=k, v=v, log_gamma=log_gamma, initial_state=initial_state)
     _check_device(name, q.device, k=k, v=v, log_gamma=log_gamma, initial_state=initial_state, cu_seqlens=cu_seqlens)
     args = (_operand(q), _operand(k), _operand(v), _decays(log_gamma),
@@ -230,6 +231,7 @@ def decay_attention_step(q, k, v, log_gamma, state, slots=None, scale: float | N
         raise ValueError(f"ttc_b200 {name}: {B} rows and {n} states")
     if (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad) and torch.is_grad_enabled():
         raise ValueError(f"ttc_b200 {name} records no gradient: call it under torch.no_grad()")
+    refuse_gradient(name, scale=scale)
     refuse_tangents(name, q=q, k=k, v=v, log_gamma=log_gamma, state=state)
     dev = q.device
     _check_device(name, dev, k=k, v=v, log_gamma=log_gamma, state=state, slots=slots)

@@ -10,7 +10,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._call import launch, on_device, refuse_tangents, wants_grad
+from ._call import launch, on_device, refuse_gradient, refuse_tangents, wants_grad
 from .decay_attention import _workspace
 from .solver import _DTYPES, _ptr
 
@@ -91,6 +91,7 @@ def group_norm(x, num_groups: int, weight=None, bias=None, gate=None, activation
     for p in params:
         if p.shape != (C,) or p.dtype not in (x.dtype, torch.float32) or p.dtype != params[0].dtype:
             raise ValueError(f"ttc_b200 group_norm: weight and bias must be [{C}] in {x.dtype} or both float32")
+    refuse_gradient("group_norm", eps=eps)
     refuse_tangents("group_norm", x=x, weight=weight, bias=bias, gate=gate)
     dev = x.device
     for t, n in ((weight, "weight"), (bias, "bias"), (gate, "gate")):

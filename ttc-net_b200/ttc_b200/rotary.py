@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._call import launch, on_device, refuse_tangents, wants_grad
+from ._call import launch, on_device, refuse_gradient, refuse_tangents, wants_grad
 from .solver import _DTYPES, _ptr
 
 
@@ -99,8 +99,9 @@ def rotary(q, k, positions, inv_freq, interleaved: bool = False, magnitude: floa
     """(q', k') for q [B, T, H, D] and k [B, T, Hk, D] (or None; float32 or bfloat16, D <= 512), turned at ``positions``
     (int32 or int64, [T] or [B, T], any values) by ``inv_freq`` [R / 2] float64: the first R <= D values of
     each head in pairs (p, p + R / 2), or (2p, 2p + 1) where ``interleaved``, multiplied by ``magnitude``; the
-    other D - R are copied.  Differentiable in q and k, once and in reverse mode.  The head dim is
-    read in place where it is contiguous, whatever the other strides."""
+    other D - R are copied.  Differentiable in q and k, once and in reverse mode (the frequencies
+    and the factor are fixed).  The head dim is read in place where it is contiguous, whatever the
+    other strides."""
     for t, n in ((q, "q"), (k, "k")):
         if t is None and n == "k":
             continue
@@ -118,7 +119,8 @@ def rotary(q, k, positions, inv_freq, interleaved: bool = False, magnitude: floa
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or 2 * inv_freq.numel() > D:
         raise ValueError(f"ttc_b200 rotary: inv_freq must be float64 [R / 2] with R <= {D}, got "
                          f"{inv_freq.dtype} {tuple(inv_freq.shape)}")
-    refuse_tangents("rotary", q=q, k=k, inv_freq=inv_freq)
+    refuse_gradient("rotary", inv_freq=inv_freq, magnitude=magnitude)
+    refuse_tangents("rotary", q=q, k=k)
     dev = q.device
     for t, n in ((k, "k"), (positions, "positions"), (inv_freq, "inv_freq")):
         if t is not None and t.device != dev:
@@ -129,5 +131,5 @@ def rotary(q, k, positions, inv_freq, interleaved: bool = False, magnitude: floa
         inv_freq = inv_freq.contiguous()
     args = (q, k, positions, inv_freq, bool(interleaved), float(magnitude))
     if wants_grad(q, k):
-        return RotaryFunction.apply(q, k, positions, inv_freq.detach(), *args[4:])
+        return RotaryFunction.apply(*args)
     return on_device(dev, _turn, *args, False)
