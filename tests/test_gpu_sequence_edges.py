@@ -1,0 +1,38 @@
+"""Calls of the sequence operators at the edges of what their documentation allows."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16]
+IDS = ["f32", "bf16"]
+
+
+def _normal(seed, *shape, dtype=torch.float32):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("B,T,Hk,H", [(1, 1, 1, 1), (1, 5, 2, 4), (1, 1, 1, 3), (3, 1, 1, 1), (2, 0, 2, 2)])
+def test_slices_of_odd_projections(B, T, Hk, H, dtype):
+    """Dims of one element (and all dims of nothing) count as contiguous whatever their strides: slices of a projection of
+    odd width, forward and backward, are what their copies are."""
+    from ttc_b200 import decay_attention, decay_attention_step
+    dk, dv = 32, 16
+    z = _normal(B + T, 3, 7, 2 * Hk * dk + H * dv + 3, dtype=dtype)[:B, :T]
+    cuts = [z[..., :Hk * dk].unflatten(-1, (Hk, dk)), z[..., Hk * dk:2 * Hk * dk].unflatten(-1, (Hk, dk)),
+            z[..., 2 * Hk * dk:2 * Hk * dk + H * dv].unflatten(-1, (H, dv))]
+    lg = torch.linspace(-0.3, -0.1, H, device="cuda")
+    start = _normal(9, B, H, dk, dv)
+    res = []
+    for ops in (cuts, [torch.empty(t.shape, dtype=dtype, device="cuda").copy_(t) for t in cuts]):
+        ins = [t.detach().requires_grad_() for t in (*ops, start)]
+        o, state = decay_attention(*ins[:3], lg, initial_state=ins[3], return_state=True)
+        grads = torch.autograd.grad((o, state), ins, (torch.ones_like(o), torch.ones_like(state)))
+        res.append([o.detach(), state.detach(), *grads])
+        if T > 0:
+            cache = start.clone()
+            res[-1] += [decay_attention_step(*(t[:, 0] for t in ops), lg, cache), cache]
+    for a, b in zip(*res):
+        assert torch.equal(a, b)

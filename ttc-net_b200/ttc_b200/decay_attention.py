@@ -62,8 +62,9 @@ _SIX, _NINE = ctypes.c_int64 * 6, ctypes.c_int64 * 9
 
 
 def _strides(t: torch.Tensor):
-    """Strides of the dims before the head dim; those of a dim of one element do not matter and may be odd."""
-    return t.stride()[:-1] if t.is_contiguous() else [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride())]
+    """Strides of the dims before the head dim, 0 where none is taken: those of a dim of one element, and all of a
+    tensor of none, may be anything, in a contiguous tensor too, and the C entries want multiples of 16 bytes."""
+    return [s if n > 1 else 0 for n, s in zip(t.shape[:-1], t.stride())] if t.numel() else [0] * (t.dim() - 1)
 
 
 def _check_qkv(name, q, k, v, log_gamma, lead):
@@ -136,7 +137,7 @@ def _backward(q, k, v, log_gamma, scale, initial_state, cu_seqlens, g_o, g_state
 def _step(q, k, v, log_gamma, scale, state, slot_stride, slots, dims):
     o = v.new_empty(v.shape)
     launch("ttc_decay_attn_step", q.device, _lib.load().ttc_decay_attn_step, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-           _SIX(*_strides(q), *_strides(k), *_strides(v)), log_gamma.data_ptr(), scale, state.data_ptr(), slot_stride,
+           _SIX(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2]), log_gamma.data_ptr(), scale, state.data_ptr(), slot_stride,
            _ptr(slots), *dims, o.data_ptr())
     return o
 
