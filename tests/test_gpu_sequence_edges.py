@@ -36,3 +36,26 @@ def test_slices_of_odd_projections(B, T, Hk, H, dtype):
             res[-1] += [decay_attention_step(*(t[:, 0] for t in ops), lg, cache), cache]
     for a, b in zip(*res):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float64])
+def test_default_dtype_changes_nothing(default):
+    from ttc_b200 import decay_attention, group_norm, rotary, rotary_frequencies
+    pos, lg = torch.arange(100, device="cuda"), torch.tensor([-0.1, -0.2], device="cuda")
+    ins = [_normal(i, 1, 100, 2, 32).requires_grad_() for i in range(3)] + [_normal(3, 1, 2, 32, 32).requires_grad_()]
+
+    def call():
+        f, _ = rotary_frequencies(32)
+        q, k = rotary(ins[0], ins[1], pos, f)
+        o, state = decay_attention(q, k, ins[2], lg, initial_state=ins[3], return_state=True)
+        y = group_norm(o.flatten(2), 2, activation="silu")
+        return [y, state, *torch.autograd.grad((y, state), ins, (torch.ones_like(y), torch.ones_like(state)))]
+
+    want = call()
+    torch.set_default_dtype(default)
+    try:
+        got = call()
+    finally:
+        torch.set_default_dtype(torch.float32)
+    for a, b in zip(got, want):
+        assert a.dtype == torch.float32 and torch.equal(a, b)

@@ -113,7 +113,7 @@ def _forward(q, k, v, log_gamma, scale, initial_state, cu_seqlens, want_state):
     dev, lib, dims = q.device, _lib.load(), _dims(q, v, cu_seqlens)
     T, n_seq, H, _, dk, dv, _ = dims
     o = v.new_empty(v.shape)
-    state = torch.empty(n_seq, H, dk, dv, device=dev) if want_state else None
+    state = torch.empty(n_seq, H, dk, dv, device=dev, dtype=torch.float32) if want_state else None
     nbytes = lib.ttc_decay_attn_workspace(T, n_seq, cu_seqlens is not None, *dims[2:], 0)
     ws = _workspace(nbytes, dev)
     launch("ttc_decay_attn_fwd", dev, lib.ttc_decay_attn_fwd, _ptr(q), _ptr(k), _ptr(v),
@@ -125,7 +125,7 @@ def _forward(q, k, v, log_gamma, scale, initial_state, cu_seqlens, want_state):
 def _backward(q, k, v, log_gamma, scale, initial_state, cu_seqlens, g_o, g_state, want_start):
     dev, lib, dims = q.device, _lib.load(), _dims(q, v, cu_seqlens)
     d_q, d_k, d_v = (t.new_empty(t.shape) for t in (q, k, v))
-    d_s = torch.empty(initial_state.shape, device=dev) if want_start else None
+    d_s = torch.empty(initial_state.shape, device=dev, dtype=torch.float32) if want_start else None
     nbytes = lib.ttc_decay_attn_workspace(*dims[:2], cu_seqlens is not None, *dims[2:], 1)
     ws = _workspace(nbytes, dev)
     launch("ttc_decay_attn_bwd", dev, lib.ttc_decay_attn_bwd, _ptr(q), _ptr(k), _ptr(v),
