@@ -59,3 +59,31 @@ def test_default_dtype_changes_nothing(default):
         torch.set_default_dtype(torch.float32)
     for a, b in zip(got, want):
         assert a.dtype == torch.float32 and torch.equal(a, b)
+
+
+def test_a_timeout_is_reported_by_a_step_and_on_request():
+    """The status word that a kernel would set, set from the host: a token's step raises and leaves its states alone."""
+    import ctypes
+    import sys
+
+    import ttc_b200
+    module = sys.modules["ttc_b200.decay_attention"]
+    q, k, v = (_normal(i, 1, 10, 2, 32, dtype=torch.bfloat16) for i in range(3))
+    lg = torch.tensor([-0.1, -0.2], device="cuda")
+    _, state = ttc_b200.decay_attention(q, k, v, lg, return_state=True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ttc_b200.decay_attention(q, k, v, lg)
+    g.replay()
+    ttc_b200.check_decay_attention()
+    word, before = ctypes.c_int.from_address(module._status_word()), state.clone()
+    word.value = 16
+    with pytest.raises(RuntimeError, match="ran out"):
+        ttc_b200.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], lg, state)
+    assert torch.equal(state, before)
+    ttc_b200.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], lg, state)
+    assert not torch.equal(state, before)
+    word.value = 16
+    with pytest.raises(RuntimeError, match="ran out"):
+        ttc_b200.check_decay_attention("cuda")
+    ttc_b200.check_decay_attention(state.device)

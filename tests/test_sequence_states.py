@@ -30,3 +30,36 @@ def test_states_are_float32_whatever_the_default_dtype(module, default):
         torch.set_default_dtype(before)
     assert state.dtype == torch.float32 and state.shape == start.shape
     assert all(t.dtype == torch.float32 for t in (o, *grads)) and grads[3].shape == start.shape
+
+
+def test_a_timeout_belongs_to_its_device(monkeypatch):
+    """Two devices' words, held in ordinary memory: a report is raised for the device that has it, once."""
+    import ctypes
+
+    import ttc_b200
+    m = sys.modules["ttc_b200.decay_attention"]
+    words = [torch.zeros(1, dtype=torch.int32) for _ in range(2)]
+    monkeypatch.setattr(m, "_status", {i: (w, ctypes.c_int.from_address(w.data_ptr())) for i, w in enumerate(words)})
+    synced = []
+    monkeypatch.setattr(torch.cuda, "synchronize", synced.append)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    assert m._status_word(0) == words[0].data_ptr() and m._status_word() == words[0].data_ptr()
+    words[1][0] = 16
+    assert m._status_word(0) == words[0].data_ptr()
+    m._raise_timeout(0)
+    m._raise_timeout(7)  # a device that had no call
+    ttc_b200.check_decay_attention()
+    with pytest.raises(RuntimeError, match="ran out.*cuda:1"):
+        m._status_word(1)
+    assert m._status_word(1) == words[1].data_ptr()
+    for device in ("cuda:1", torch.device("cuda", 1), 1):
+        words[1][0] = 16
+        with pytest.raises(RuntimeError, match="ran out.*cuda:1"):
+            ttc_b200.check_decay_attention(device)
+        ttc_b200.check_decay_attention(device)
+    assert synced == [0] + [1] * 6
+    q, state = torch.zeros(1, 1, 8), torch.zeros(1, 1, 8, 8)
+    q_on_1 = type("OnOne", (), {"device": torch.device("cuda", 1), "new_empty": None})
+    words[1][0] = 16
+    with pytest.raises(RuntimeError, match="ran out.*cuda:1"):  # a token's step, before anything else
+        m._step(q_on_1, q, q, None, 1.0, state, 64, None, ())

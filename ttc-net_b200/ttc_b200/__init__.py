@@ -8,7 +8,7 @@ The solver is libttc_b200.so (include/ttc_b200.h), bound with ctypes.  Beside th
 no tokens, stand the operators of a memory over them: ``decay_attention`` (prompts and training),
 ``decay_attention_step`` (one token over a cache of states), ``rotary`` and ``group_norm``.
 """
-from .decay_attention import decay_attention, decay_attention_step
+from .decay_attention import check_decay_attention, decay_attention, decay_attention_step
 from .group_norm import group_norm
 from .layer import TTCLayer, l2norm
 from .rotary import rotary, rotary_frequencies
@@ -18,4 +18,4 @@ from .trajectory import lqr_trajectory
 
 __all__ = ["TTCLayer", "LQR_SOLVER_IMPL_MAP", "LQRSolveFunction", "cuda_lqr_solve",
            "fused_lqr_solve", "kkt_lqr_solve", "lqr_solve_with_status", "lqr_trajectory", "l2norm",
-           "decay_attention", "decay_attention_step", "rotary", "rotary_frequencies", "group_norm"]
+           "decay_attention", "decay_attention_step", "check_decay_attention", "rotary", "rotary_frequencies", "group_norm"]

@@ -27,24 +27,41 @@ def _workspace(nbytes: int, dev) -> torch.Tensor | None:
     return torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
 
 
-# One word of pinned host memory that every kernel can reach: it is read at the next call without
-# waiting for the GPU.
-_status: torch.Tensor | None = None
+# For each device one word of pinned host memory that its kernels can reach, and a view of it: it is read at
+# the next call without waiting for the GPU.
+_status: dict[int, tuple[torch.Tensor, ctypes.c_int]] = {}
 
 WAIT_TIMEOUT_MSG = ("ttc_b200 decay_attention: a wait inside an earlier call's kernel ran out "
                     "(that call's results are not valid)")
 
 
-def _status_word() -> int:
-    """The address of the status word; raises if a call since the last one reported a timeout."""
-    global _status
-    if _status is None:
-        _status = torch.zeros(1, dtype=torch.int32, pin_memory=True)
-    word = ctypes.c_int.from_address(_status.data_ptr())
-    if word.value:
-        word.value = 0
-        raise RuntimeError(WAIT_TIMEOUT_MSG)
-    return _status.data_ptr()
+def _raise_timeout(device: int) -> None:
+    """Raises if a call on the device reported a timeout since the last time this raised."""
+    held = _status.get(device)
+    if held is not None and held[1].value:
+        held[1].value = 0
+        raise RuntimeError(f"{WAIT_TIMEOUT_MSG[:-1]}, on cuda:{device})")
+
+
+def _status_word(device: int | None = None) -> int:
+    """The address of the device's status word (None: of the current device's); raises as `_raise_timeout`."""
+    device = torch.cuda.current_device() if device is None else device
+    if device not in _status:
+        word = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+        _status.setdefault(device, (word, ctypes.c_int.from_address(word.data_ptr())))
+    _raise_timeout(device)
+    return _status[device][0].data_ptr()
+
+
+def check_decay_attention(device=None) -> None:
+    """Waits for the device (None: the current one) and raises RuntimeError if a wait inside a
+    ``decay_attention`` kernel ran out on it since the last report; that call's results, and states that went
+    on from them, are not valid.  Calls report it by themselves, but only what was known when they were made:
+    ask here behind replays of a captured call and before results leave the program."""
+    device = torch.cuda.current_device() if device is None else torch.device(device).index
+    device = torch.cuda.current_device() if device is None else device
+    torch.cuda.synchronize(device)
+    _raise_timeout(device)
 
 
 def _operand(t: torch.Tensor) -> torch.Tensor:
@@ -111,30 +128,34 @@ def _dims(q, v, cu_seqlens):
 
 def _forward(q, k, v, log_gamma, scale, initial_state, cu_seqlens, want_state):
     dev, lib, dims = q.device, _lib.load(), _dims(q, v, cu_seqlens)
+    status = _status_word(dev.index)
     T, n_seq, H, _, dk, dv, _ = dims
     o = v.new_empty(v.shape)
     state = torch.empty(n_seq, H, dk, dv, device=dev, dtype=torch.float32) if want_state else None
     nbytes = lib.ttc_decay_attn_workspace(T, n_seq, cu_seqlens is not None, *dims[2:], 0)
     ws = _workspace(nbytes, dev)
     launch("ttc_decay_attn_fwd", dev, lib.ttc_decay_attn_fwd, _ptr(q), _ptr(k), _ptr(v),
-           _NINE(*_strides(q), *_strides(k), *_strides(v)), _ptr(log_gamma), scale, _ptr(initial_state), _ptr(cu_seqlens), *dims, _ptr(o), _ptr(state), _ptr(ws), nbytes,
-           _status_word())
+           _NINE(*_strides(q), *_strides(k), *_strides(v)), _ptr(log_gamma), scale,
+           _ptr(initial_state), _ptr(cu_seqlens), *dims, _ptr(o), _ptr(state), _ptr(ws), nbytes, status)
     return o, state
 
 
 def _backward(q, k, v, log_gamma, scale, initial_state, cu_seqlens, g_o, g_state, want_start):
     dev, lib, dims = q.device, _lib.load(), _dims(q, v, cu_seqlens)
+    status = _status_word(dev.index)
     d_q, d_k, d_v = (t.new_empty(t.shape) for t in (q, k, v))
     d_s = torch.empty(initial_state.shape, device=dev, dtype=torch.float32) if want_start else None
     nbytes = lib.ttc_decay_attn_workspace(*dims[:2], cu_seqlens is not None, *dims[2:], 1)
     ws = _workspace(nbytes, dev)
     launch("ttc_decay_attn_bwd", dev, lib.ttc_decay_attn_bwd, _ptr(q), _ptr(k), _ptr(v),
-           _NINE(*_strides(q), *_strides(k), *_strides(v)), _ptr(g_o), _ptr(log_gamma), scale, _ptr(initial_state), _ptr(g_state), _ptr(cu_seqlens), *dims, _ptr(d_q), _ptr(d_k),
-           _ptr(d_v), _ptr(d_s), _ptr(ws), nbytes, _status_word())
+           _NINE(*_strides(q), *_strides(k), *_strides(v)), _ptr(g_o), _ptr(log_gamma), scale,
+           _ptr(initial_state), _ptr(g_state), _ptr(cu_seqlens), *dims, _ptr(d_q), _ptr(d_k), _ptr(d_v), _ptr(d_s),
+           _ptr(ws), nbytes, status)
     return d_q, d_k, d_v, d_s
 
 
 def _step(q, k, v, log_gamma, scale, state, slot_stride, slots, dims):
+    _raise_timeout(q.device.index)  # before the states advance
     o = v.new_empty(v.shape)
     launch("ttc_decay_attn_step", q.device, _lib.load().ttc_decay_attn_step, q.data_ptr(), k.data_ptr(), v.data_ptr(),
            _SIX(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2]), log_gamma.data_ptr(), scale, state.data_ptr(), slot_stride,
