@@ -87,3 +87,59 @@ def test_a_timeout_is_reported_by_a_step_and_on_request():
     with pytest.raises(RuntimeError, match="ran out"):
         ttc_b200.check_decay_attention("cuda")
     ttc_b200.check_decay_attention(state.device)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("Hk", [1, 2])
+def test_losses_on_some_of_the_outputs(monkeypatch, Hk, dtype):
+    """Of (o, state): a loss on one is a loss on both with zeros for the other, and what is not there reaches the C
+    entry as NULL."""
+    import sys
+
+    from ttc_b200 import decay_attention
+    module = sys.modules["ttc_b200.decay_attention"]
+    lg, seen, backward = torch.tensor([-0.1, -0.2], device="cuda"), [], module._backward
+
+    def spy(*args):
+        seen.append(args[8] is not None)  # the last state's gradient
+        return backward(*args)
+
+    monkeypatch.setattr(module, "_backward", spy)
+    ins = [_normal(i, 2, 70, h, 32, dtype=dtype).requires_grad_() for i, h in enumerate((Hk, Hk, 2))]
+    ins.append(_normal(7, 2, 2, 32, 32).requires_grad_())
+    go, gs = _normal(8, 2, 70, 2, 32, dtype=dtype), _normal(9, 2, 2, 32, 32)
+
+    def grads(outs, gos):
+        o, state = decay_attention(*ins[:3], lg, initial_state=ins[3], return_state=True)
+        return torch.autograd.grad([(o, state)[i] for i in outs], ins, gos)
+
+    for outs, gos, both in (([0], [go], [go, torch.zeros_like(gs)]), ([1], [gs], [torch.zeros_like(go), gs])):
+        for a, b in zip(grads(outs, gos), grads([0, 1], both)):
+            assert torch.equal(a, b)
+    assert seen == [False, True, True, True]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_losses_on_one_of_rotarys_outputs(dtype):
+    from ttc_b200 import rotary, rotary_frequencies
+    f, _ = rotary_frequencies(32)
+    ins = [_normal(i, 2, 9, h, 32, dtype=dtype).requires_grad_() for i, h in enumerate((4, 2))]
+    g = [_normal(5 + i, *t.shape, dtype=dtype) for i, t in enumerate(ins)]
+    pos = torch.arange(9, device="cuda")
+    want = torch.autograd.grad(rotary(*ins, pos, f), ins, g)
+    for i in range(2):
+        got = torch.autograd.grad(rotary(*ins, pos, f)[i], ins, g[i])
+        assert torch.equal(got[i], want[i]) and got[1 - i].dtype == dtype and torch.equal(got[1 - i], torch.zeros_like(ins[1 - i]))
+    # neither: an operator behind them that forms no gradient
+
+    class Nothing(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, a, b):
+            return a.sum()
+
+        @staticmethod
+        def backward(ctx, g):
+            return None, None
+
+    for x in torch.autograd.grad(Nothing.apply(*rotary(*ins, pos, f)), ins, allow_unused=True):
+        assert x is None

@@ -168,6 +168,7 @@ class DecayAttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, log_gamma, scale, initial_state, cu_seqlens, want_state):
+        ctx.set_materialize_grads(False)  # None for an output that the loss does not see, a state's above all
         ctx.save_for_backward(q, k, v, log_gamma, initial_state, cu_seqlens)
         ctx.scale = scale
         return on_device(q.device, _forward, q, k, v, log_gamma, scale, initial_state, cu_seqlens, want_state)
@@ -176,6 +177,8 @@ class DecayAttentionFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g_o, g_state):
         refuse_tangents("decay_attention", g_o=g_o, g_state=g_state)
+        if g_o is None and g_state is None:
+            return (None,) * 8
         q, k, v, log_gamma, initial_state, cu_seqlens = ctx.saved_tensors
         g_o = torch.zeros_like(v) if g_o is None else g_o
         g_o = _aligned(g_o.contiguous())

@@ -76,6 +76,7 @@ class RotaryFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, interleaved, magnitude):
+        ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions, inv_freq)
         ctx.how = (interleaved, magnitude)
         ctx.like = q.shape, None if k is None else k.shape, q.dtype
@@ -85,13 +86,18 @@ class RotaryFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g_q, g_k):
         refuse_tangents("rotary", g_q=g_q, g_k=g_k)
+        if g_q is None and g_k is None:
+            return (None,) * 6
         positions, inv_freq = ctx.saved_tensors
         q_shape, k_shape, dtype = ctx.like
-        if g_q is None:
-            g_q = torch.zeros(q_shape, dtype=dtype, device=positions.device)
-        if g_k is None and k_shape is not None:
-            g_k = torch.zeros(k_shape, dtype=dtype, device=positions.device)
-        d_q, d_k = on_device(positions.device, _turn, g_q, g_k, positions, inv_freq, *ctx.how, True)
+        # what the loss sees is turned back, the other's gradient is zeros
+        some, other = (g_k, None) if g_q is None else (g_q, g_k)
+        d_some, d_other = on_device(positions.device, _turn, some, other, positions, inv_freq, *ctx.how, True)
+        d_q, d_k = (None, d_some) if g_q is None else (d_some, d_other)
+        if d_q is None:
+            d_q = torch.zeros(q_shape, dtype=dtype, device=positions.device)
+        if d_k is None and k_shape is not None:
+            d_k = torch.zeros(k_shape, dtype=dtype, device=positions.device)
         return d_q, d_k, None, None, None, None
 
 
