@@ -143,3 +143,26 @@ def test_losses_on_one_of_rotarys_outputs(dtype):
 
     for x in torch.autograd.grad(Nothing.apply(*rotary(*ins, pos, f)), ins, allow_unused=True):
         assert x is None
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("T", [5, 1500])
+def test_decays_that_are_not_numbers_show(T, dtype):
+    """gamma = NaN: S_0 = NaN 0 + k v and all that follows, of this head alone; not the head without memory that a
+    logarithm of -inf is."""
+    from ttc_b200 import decay_attention, decay_attention_step
+    q, k, v = (_normal(i, 1, T, 3, 32, dtype=dtype) for i in range(3))
+    lg, clean = torch.tensor([-0.1, float("nan"), -0.2], device="cuda"), torch.tensor([-0.1, -0.3, -0.2], device="cuda")
+    res = []
+    for x in (lg, clean):
+        ins = [t.detach().requires_grad_() for t in (q, k, v)]
+        o, state = decay_attention(*ins, x, return_state=True)
+        step = state.detach().clone()
+        one = decay_attention_step(q[:, 0], k[:, 0], v[:, 0], x, step)
+        res.append([o.detach(), *torch.autograd.grad(o, ins, torch.ones_like(o)), state.detach().transpose(0, 1)[None],
+                    one[:, None], step.transpose(0, 1)[None]])
+    for i, (a, b) in enumerate(zip(*res)):  # heads are dim 2, of the states dim 1
+        a, b = (a, b) if i not in (4, 6) else (a.transpose(1, 2), b.transpose(1, 2))
+        assert torch.isnan(a[:, :, 1]).all()
+        for h in (0, 2):
+            assert torch.equal(a[:, :, h], b[:, :, h])

@@ -137,9 +137,9 @@ __device__ __forceinline__ Item find_item(const Args& A, int x) {
 }
 
 // gamma^n; log gamma = -inf (no memory) is taken as -1e4, whose powers are 0 from n = 1 on and
-// 1 at n = 0.
+// 1 at n = 0.  A comparison, not fmaxf, which would make -1e4 of a NaN too.
 __device__ __forceinline__ float decay_pow(float lg, int64_t n) {
-  return static_cast<float>(exp(static_cast<double>(fmaxf(lg, -1e4f)) * static_cast<double>(n)));
+  return static_cast<float>(exp(static_cast<double>(lg < -1e4f ? -1e4f : lg) * static_cast<double>(n)));
 }
 
 // Zeros in the rows behind the last packed sequence.
