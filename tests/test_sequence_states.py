@@ -63,3 +63,14 @@ def test_a_timeout_belongs_to_its_device(monkeypatch):
     words[1][0] = 16
     with pytest.raises(RuntimeError, match="ran out.*cuda:1"):  # a token's step, before anything else
         m._step(q_on_1, q, q, None, 1.0, state, 64, None, ())
+
+
+def test_sizes_of_packed_rows_are_the_rows(module):
+    """A packed row has T tokens in all: a long one of many sequences is no larger than its blocks and sequences."""
+    from ttc_b200 import _lib
+    size = _lib.load().ttc_decay_attn_workspace
+    assert size(1 << 21, 131000, 1, 8, 8, 16, 16, _lib.DTYPE_BF16, 0) == 0
+    assert size(1 << 28, 1000, 1, 8, 8, 16, 16, _lib.DTYPE_F32, 0) == 0
+    assert size((1 << 31) - 65, 1 << 20, 1, 1, 1, 16, 16, _lib.DTYPE_F32, 0) == -_lib.ERR_INVALID  # sequences x heads
+    assert size(1 << 21, 131000, 0, 8, 8, 16, 16, _lib.DTYPE_BF16, 0) == -_lib.ERR_INVALID  # 2^38 tokens
+    assert size((1 << 31) - 65, 1000, 1, 8, 8, 16, 16, _lib.DTYPE_F32, 0) == 0

@@ -267,7 +267,7 @@ Plan plan(int64_t T, int n_seq, bool packed, int H, int dk, int dv, int passes, 
 // Whether any sequence may have more than one segment.
 bool segmented(const Plan& p, int64_t T) { return p.seg_len < T; }
 
-int check(int64_t T, int n_seq, int H, int Hk, int dk, int dv, int dtype) {
+int check(int64_t T, int n_seq, bool packed, int H, int Hk, int dk, int dv, int dtype) {
   if (T < 0 || T > 0x7fffffffLL - C || n_seq < 0) return fail(TTC_ERR_INVALID, "decay_attn: tokens must be in [0, 2^31 - 64), sequences >= 0");
   if (H < 1 || H > 65535 || Hk < 1 || H % Hk != 0)
     return fail(TTC_ERR_INVALID, "decay_attn: heads must be in [1, 65535] and a multiple of the key heads");
@@ -275,9 +275,11 @@ int check(int64_t T, int n_seq, int H, int Hk, int dk, int dv, int dtype) {
     return fail(TTC_ERR_INVALID, "decay_attn: dtype must be TTC_DTYPE_F32 or TTC_DTYPE_BF16");
   if (dk < 8 || dk > 128 || dk % 8 || dv < 8 || dv > 128 || dv % 8)
     return fail(TTC_ERR_UNSUPPORTED, "decay_attn: head dims must be multiples of 8 from 8 to 128");
-  const int64_t most = 0x7fffffffLL;
-  if (static_cast<int64_t>(n_seq) * H > 65535 * 16LL || (T / C + 1) * n_seq > most)
+  if (static_cast<int64_t>(n_seq) * H > 65535 * 16LL)
     return fail(TTC_ERR_INVALID, "decay_attn: too many sequences x heads (at most 2^20 - 16)");
+  // (a packed row of 2^31 tokens has 2^25 blocks and at most one more for each sequence)
+  if (!packed && (T / C + 1) * n_seq > 0x7fffffffLL)
+    return fail(TTC_ERR_INVALID, "decay_attn: too many blocks of 64 tokens (at most 2^31 - 1)");
   return TTC_OK;
 }
 
@@ -334,7 +336,7 @@ using namespace ttc;
 
 extern "C" int64_t ttc_decay_attn_workspace(int64_t T, int n_seq, int packed, int H, int Hk, int dk, int dv, int dtype,
                                             int backward) {
-  if (int rc = da::check(T, n_seq, H, Hk, dk, dv, dtype)) return -rc;
+  if (int rc = da::check(T, n_seq, packed != 0, H, Hk, dk, dv, dtype)) return -rc;
   if (n_seq == 0) return 0;
   const int passes = backward ? 3 : 1;
   int64_t bytes = da::state_bytes(da::plan(T, n_seq, packed != 0, H, dk, dv, passes, dtype), T, H, dk, dv, passes);
@@ -347,7 +349,7 @@ extern "C" int ttc_decay_attn_fwd(const void* q, const void* k, const void* v, c
                                   const int* cu_seqlens, int64_t T, int n_seq, int H, int Hk, int dk, int dv, int dtype,
                                   void* o, float* final_state, void* workspace, int64_t workspace_bytes, int* status,
                                   void* stream) {
-  if (int rc = da::check(T, n_seq, H, Hk, dk, dv, dtype)) return rc;
+  if (int rc = da::check(T, n_seq, cu_seqlens != nullptr, H, Hk, dk, dv, dtype)) return rc;
   if (n_seq == 0) return cu_seqlens ? da::fail(TTC_ERR_INVALID, "decay_attn: packed rows need a sequence") : TTC_OK;
   if (!strides || !log_gamma || (T > 0 && (!q || !k || !v || !o)))
     return da::fail(TTC_ERR_INVALID, "decay_attn_fwd: null pointer");
@@ -388,7 +390,7 @@ extern "C" int ttc_decay_attn_bwd(const void* q, const void* k, const void* v, c
                                   const float* g_final_state, const int* cu_seqlens, int64_t T, int n_seq, int H, int Hk,
                                   int dk, int dv, int dtype, void* d_q, void* d_k, void* d_v, float* d_initial_state,
                                   void* workspace, int64_t workspace_bytes, int* status, void* stream) {
-  if (int rc = da::check(T, n_seq, H, Hk, dk, dv, dtype)) return rc;
+  if (int rc = da::check(T, n_seq, cu_seqlens != nullptr, H, Hk, dk, dv, dtype)) return rc;
   if (n_seq == 0) return cu_seqlens ? da::fail(TTC_ERR_INVALID, "decay_attn: packed rows need a sequence") : TTC_OK;
   if (!strides || !log_gamma || (T > 0 && (!q || !k || !v || !g_o || !d_q || !d_k || !d_v)))
     return da::fail(TTC_ERR_INVALID, "decay_attn_bwd: null pointer");
@@ -466,7 +468,7 @@ extern "C" int ttc_decay_attn_step(const void* q, const void* k, const void* v, 
                                    const float* log_gamma, float scale, float* state, int64_t slot_stride,
                                    const int* slots, int B, int n_slots, int H, int Hk, int dk, int dv, int dtype,
                                    void* o, void* stream) {
-  if (int rc = da::check(1, B, H, Hk, dk, dv, dtype)) return rc;
+  if (int rc = da::check(1, B, false, H, Hk, dk, dv, dtype)) return rc;
   if (n_slots < 0 || (!slots && n_slots < B)) return da::fail(TTC_ERR_INVALID, "decay_attn_step: fewer states than rows");
   if (B == 0) return TTC_OK;
   if (!q || !k || !v || !strides || !log_gamma || !o || (n_slots > 0 && !state))
