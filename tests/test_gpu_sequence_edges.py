@@ -166,3 +166,22 @@ def test_decays_that_are_not_numbers_show(T, dtype):
         assert torch.isnan(a[:, :, 1]).all()
         for h in (0, 2):
             assert torch.equal(a[:, :, h], b[:, :, h])
+
+
+def test_default_device_changes_nothing(monkeypatch):
+    """A program that builds its tensors on the GPU by default, from its first call on."""
+    import sys
+
+    import ttc_b200
+    monkeypatch.setattr(sys.modules["ttc_b200.decay_attention"], "_status", {})
+    q, k, v = (_normal(i, 1, 10, 2, 32, dtype=torch.bfloat16) for i in range(3))
+    lg, pos = torch.tensor([-0.1, -0.2], device="cuda"), torch.arange(10, device="cuda")
+
+    def call():
+        f, _ = ttc_b200.rotary_frequencies(32, scaling="yarn", factor=2.0, original_length=100)
+        a, b = ttc_b200.rotary(q, k, pos, f)
+        return ttc_b200.group_norm(ttc_b200.decay_attention(a, b, v, lg).flatten(2), 2)
+
+    with torch.device("cuda"):
+        got = call()
+    assert torch.equal(got, call())

@@ -47,7 +47,7 @@ def _status_word(device: int | None = None) -> int:
     """The address of the device's status word (None: of the current device's); raises as `_raise_timeout`."""
     device = torch.cuda.current_device() if device is None else device
     if device not in _status:
-        word = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+        word = torch.zeros(1, dtype=torch.int32, device="cpu", pin_memory=True)
         _status.setdefault(device, (word, ctypes.c_int.from_address(word.data_ptr())))
     _raise_timeout(device)
     return _status[device][0].data_ptr()

@@ -33,7 +33,7 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: str = "none
         raise ValueError(f"rotary_frequencies: unknown scaling {scaling!r}")
     if not (factor > 0 and base > 0):
         raise ValueError("rotary_frequencies: base and factor must be positive")
-    p = torch.arange(rot_dim // 2, dtype=torch.float64)
+    p = torch.arange(rot_dim // 2, dtype=torch.float64, device="cpu")
     if scaling == "ntk" and rot_dim > 2:
         base = base * factor ** (rot_dim / (rot_dim - 2.0))
     f = float(base) ** (-2.0 * p / rot_dim)
