@@ -185,3 +185,27 @@ def test_default_device_changes_nothing(monkeypatch):
     with torch.device("cuda"):
         got = call()
     assert torch.equal(got, call())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("T", [61, 8192, 30001])
+@pytest.mark.parametrize("H,Hk,dk,dv", [(3, 3, 16, 40), (4, 2, 128, 64)])
+def test_many_rows_behind_the_last_sequence(H, Hk, dk, dv, T, dtype):
+    """A buffer of fixed size with a few rows in use: zeros behind them, in o and in every gradient, in memory that held
+    something else, and the rows in use as they are alone."""
+    from ttc_b200 import decay_attention
+    cu = torch.tensor([0, 7, 7, 50], dtype=torch.int32, device="cuda")
+    lg = torch.linspace(-0.3, -0.1, H, device="cuda")
+    ins = [_normal(i, 1, T, h, d, dtype=dtype).requires_grad_() for i, (h, d) in enumerate(((Hk, dk), (Hk, dk), (H, dv)))]
+    go = _normal(5, 1, T, H, dv, dtype=dtype)
+
+    def call(ts, go):
+        o = decay_attention(*ts, lg, cu_seqlens=cu)
+        return [o.detach(), *torch.autograd.grad(o, ts, go)]
+
+    want = call([t.detach()[:, :50].requires_grad_() for t in ins], go[:, :50])
+    stale = [torch.full_like(t, float("nan")) for t in (*ins, *ins, go, go)]
+    torch.cuda.synchronize()
+    del stale  # what the outputs are allocated from
+    for a, b in zip(call(ins, go), want):
+        assert torch.equal(a[:, :50], b) and (a[:, 50:] == 0).all()

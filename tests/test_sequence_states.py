@@ -74,3 +74,19 @@ def test_sizes_of_packed_rows_are_the_rows(module):
     assert size((1 << 31) - 65, 1 << 20, 1, 1, 1, 16, 16, _lib.DTYPE_F32, 0) == -_lib.ERR_INVALID  # sequences x heads
     assert size(1 << 21, 131000, 0, 8, 8, 16, 16, _lib.DTYPE_BF16, 0) == -_lib.ERR_INVALID  # 2^38 tokens
     assert size((1 << 31) - 65, 1000, 1, 8, 8, 16, 16, _lib.DTYPE_F32, 0) == 0
+
+
+def test_outputs_off_the_16_byte_grid_are_rejected():
+    """Before any launch: the pointers are never read."""
+    import ctypes
+
+    from ttc_b200 import _lib
+    lib, strides = _lib.load(), (ctypes.c_int64 * 9)(*[64] * 9)
+    for dtype in (_lib.DTYPE_F32, _lib.DTYPE_BF16):
+        assert lib.ttc_decay_attn_fwd(16, 16, 16, strides, 16, 1.0, None, None, 8, 1, 4, 4, 16, 16, dtype, 8, None, None, 0, None,
+                                      None) == _lib.ERR_INVALID
+        for at in range(3):
+            outs = [16 if i != at else 24 for i in range(3)]
+            assert lib.ttc_decay_attn_bwd(16, 16, 16, strides, 16, 16, 1.0, None, None, None, 8, 1, 4, 4, 16, 16, dtype, *outs, None,
+                                          None, 0, None, None) == _lib.ERR_INVALID
+        assert b"aligned" in lib.ttc_last_error()

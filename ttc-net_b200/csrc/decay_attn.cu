@@ -356,6 +356,7 @@ extern "C" int ttc_decay_attn_fwd(const void* q, const void* k, const void* v, c
   const void* ops[3] = {q, k, v};
   for (int i = 0; i < 3; ++i)
     if (int rc = da::check_operand(ops[i], strides + 3 * i, 3, dtype)) return rc;
+  if (da::misaligned16(o)) return da::fail(TTC_ERR_INVALID, "decay_attn_fwd: o must be 16-byte aligned");
   const da::Plan p = da::plan(T, n_seq, cu_seqlens != nullptr, H, dk, dv, 1, dtype);
   const int64_t need = da::state_bytes(p, T, H, dk, dv, 1);
   if (workspace_bytes < need || (need > 0 && (!workspace || da::misaligned16(workspace))))
@@ -399,6 +400,8 @@ extern "C" int ttc_decay_attn_bwd(const void* q, const void* k, const void* v, c
     if (int rc = da::check_operand(ops[i], strides + 3 * i, 3, dtype)) return rc;
   const int64_t gs[3] = {T * H * dv, static_cast<int64_t>(H) * dv, dv};
   if (int rc = da::check_operand(g_o, gs, 0, dtype)) return rc;
+  if (da::misaligned16(d_q) || da::misaligned16(d_k) || da::misaligned16(d_v))
+    return da::fail(TTC_ERR_INVALID, "decay_attn_bwd: d_q, d_k and d_v must be 16-byte aligned");
   const da::Plan p = da::plan(T, n_seq, cu_seqlens != nullptr, H, dk, dv, 3, dtype);
   const int64_t sbytes = da::state_bytes(p, T, H, dk, dv, 3);
   const int grp = H / Hk;

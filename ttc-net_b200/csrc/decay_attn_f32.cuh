@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kF32Threads, (DK + DV <= 64 ? 2 : 1)) decay_at
   char* const Ps = smem + S::QB + S::KB + S::VB;
   float* const pw = reinterpret_cast<float*>(Ps + S::PB);
 
-  if (!STATE_ONLY && A.cu != nullptr && static_cast<int>(blockIdx.x) == A.items) {
+  if (!STATE_ONLY && A.cu != nullptr && static_cast<int>(blockIdx.x) >= A.items) {
     zero_rows_behind<false>(A, P, h, tid, kF32Threads);
     return;
   }

@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_attn_tc_kernel(const __gr
   const int h = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
-  if (!STATE_ONLY && A.cu != nullptr && static_cast<int>(blockIdx.x) == A.items) {
+  if (!STATE_ONLY && A.cu != nullptr && static_cast<int>(blockIdx.x) >= A.items) {
     zero_rows_behind<true>(A, P, h, tid, kTcThreads);
     return;
   }

@@ -96,7 +96,7 @@ int launch_tc_shape(const Args& A, int passes, int* status, cudaStream_t st) {
     return set_error(TTC_ERR_UNSUPPORTED, "decay_attn_tc_kernel: built with fewer than 96 registers a thread");
   if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e == cudaSuccess) {
-    const unsigned x = static_cast<unsigned>(A.items) + (!STATE_ONLY && A.cu != nullptr ? 1u : 0u);
+    const unsigned x = static_cast<unsigned>(A.items) + clearing_ctas(A, STATE_ONLY);
     k<<<dim3(x, static_cast<unsigned>(A.H), static_cast<unsigned>(passes)), kTcThreads, smem, st>>>(A, M, status);
     e = cudaGetLastError();
   }

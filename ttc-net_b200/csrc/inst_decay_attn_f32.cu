@@ -11,8 +11,7 @@ int launch_f32_shape(const Args& A, int passes, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
   if (S::SMEM > 48 * 1024) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
   if (e == cudaSuccess) {
-    // packed rows: one more CTA a head for the rows behind the last sequence
-    const unsigned x = static_cast<unsigned>(A.items) + (!STATE_ONLY && A.cu != nullptr ? 1u : 0u);
+    const unsigned x = static_cast<unsigned>(A.items) + clearing_ctas(A, STATE_ONLY);
     k<<<dim3(x, static_cast<unsigned>(A.H), static_cast<unsigned>(passes)), kF32Threads, S::SMEM, st>>>(A);
     e = cudaGetLastError();
   }
