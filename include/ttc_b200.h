@@ -301,7 +301,8 @@ int ttc_prologue_bwd(const void* Z, int64_t N, int nh, int d, int du, int rB, in
  * multiple of 16 bytes; the head dims are contiguous and every pointer is 16-byte aligned.
  * Outputs, g_o and states are contiguous: o, g_o, d_v [.., H, dv], d_q, d_k [.., Hk, dk], states
  * [n_seq, H, dk, dv] float32.  initial_state, final_state, g_final_state and
- * d_initial_state may be NULL.
+ * d_initial_state may be NULL.  At most 2^31 - 65 tokens in a row, 2^20 - 16 sequences times heads (rows times
+ * heads in the step).
  * workspace: ttc_decay_attn_workspace(...) bytes (T, n_seq, packed as above; minus an error code
  * for bad sizes), 16-byte aligned, not shared by calls that may overlap; its contents need not be kept
  * between the forward and the backward.

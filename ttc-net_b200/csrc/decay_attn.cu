@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) shared_heads_kernel(const float* __restri
 // of every R-th state row (16-byte accesses, up to 8 loads in flight), the rows' parts of o are
 // added in shared memory.  Rows of one slot are consecutive tokens of it: the CTA of the first
 // such row takes them all in order and the others leave, so no two CTAs touch one state.
-// 64 rows of 32 heads of 128 x 128 (268 MB of states): 43 us, 6.2 TB/s or 0.95 of the copy rate.
+// 64 rows of 32 heads of 128 x 128 (268 MB of states): 49 us, 5.5 TB/s or 0.84 of the copy rate.
 template <typename T>
 __global__ void __launch_bounds__(256)
     decay_attn_step_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, int64_t qsb,
@@ -217,10 +217,13 @@ struct Plan {
 // How a call is split: one CTA for each (sequence, head, pass), or sequences cut into segments whose states
 // are summed first (a second pass over k and v) and joined by a scan.  The least cost over the number of segments decides,
 // segments have at least four blocks.  In units of a block's time on one CTA (1.9 us in bf16 at 128 x 128, 1.5 at
-// 64 x 64; in fp32 7 us at 32 x 64, 9 at 64 x 64), `rounds` of CTAs over the SMs cost their segment's blocks and
+// 64 x 64; in fp32 7 us at 32 x 64, 9 at 64 x 64; one set of costs for all widths), `rounds` of CTAs over the SMs cost their segment's blocks and
 // `start` for a CTA's beginning and end; those of the sums `sum` of the blocks and `sum_start`; `more` is for the two
 // further launches, `state` for the trips of one segment's 128 x 128 state through memory.  Fitted to measured times: 8192
-// tokens, 32 heads of 128: 224 us as one, 134 in 4 segments, 187 in 9; 2 x 4096: 116 as one, 129 in 2.
+// tokens, 32 heads of 128: 224 us as one, 134 in 4 segments, 187 in 9; 2 x 4096: 116 as one, 129 in 2.  A backward counts as one
+// launch of three passes, also where unequal widths of dk and dv make it two, of 2 / 3 and 1 / 3 of the CTAs.  Packed rows are cut
+// by their number alone, the lengths being on the device: one long prompt among three short ones, 32 heads of 128,
+// 32 768 tokens, is not (957 us).
 struct Costs {
   double start, sum, sum_start, more, state;
 };
@@ -268,7 +271,8 @@ Plan plan(int64_t T, int n_seq, bool packed, int H, int dk, int dv, int passes, 
 bool segmented(const Plan& p, int64_t T) { return p.seg_len < T; }
 
 int check(int64_t T, int n_seq, bool packed, int H, int Hk, int dk, int dv, int dtype) {
-  if (T < 0 || T > 0x7fffffffLL - C || n_seq < 0) return fail(TTC_ERR_INVALID, "decay_attn: tokens must be in [0, 2^31 - 64), sequences >= 0");
+  if (T < 0 || T > 0x7fffffffLL - C || n_seq < 0)
+    return fail(TTC_ERR_INVALID, "decay_attn: tokens must be in [0, 2^31 - 64), sequences >= 0");
   if (H < 1 || H > 65535 || Hk < 1 || H % Hk != 0)
     return fail(TTC_ERR_INVALID, "decay_attn: heads must be in [1, 65535] and a multiple of the key heads");
   if (dtype != TTC_DTYPE_F32 && dtype != TTC_DTYPE_BF16)

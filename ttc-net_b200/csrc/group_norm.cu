@@ -143,8 +143,9 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, const float2 (&v)[4]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
 }
 
-// sigmoid(u).  For bf16 outputs with the approximate exponential and reciprocal, off by a few 2^-22 (the
-// result is rounded to 2^-8); their exact forms were half of the kernels' instructions.
+// sigmoid(u).  For bf16 outputs with the approximate exponential and reciprocal, off by up to (4 + 1.2 |u|) 2^-23 (10^-5
+// at u = -88, where u sigmoid(u) is 10^-36; the result is rounded to 2^-8); their exact forms were half of the
+// kernels' instructions.
 template <typename T>
 __device__ __forceinline__ float sigmoid(float u) {
   if constexpr (sizeof(T) == 2) {

@@ -158,8 +158,8 @@ def _step(q, k, v, log_gamma, scale, state, slot_stride, slots, dims):
     _raise_timeout(q.device.index)  # before the states advance
     o = v.new_empty(v.shape)
     launch("ttc_decay_attn_step", q.device, _lib.load().ttc_decay_attn_step, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-           _SIX(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2]), log_gamma.data_ptr(), scale, state.data_ptr(), slot_stride,
-           _ptr(slots), *dims, o.data_ptr())
+           _SIX(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2]), log_gamma.data_ptr(), scale,
+           state.data_ptr(), slot_stride, _ptr(slots), *dims, o.data_ptr())
     return o
 
 
@@ -204,8 +204,16 @@ def decay_attention(q, k, v, log_gamma, scale: float | None = None, initial_stat
     sequence i the tokens cu_seqlens[i] .. cu_seqlens[i + 1] - 1; states are [n, H, dk, dv].  Rows
     behind the last sequence get zeros.  Offsets past the row are cut to it.
 
-    A token's output depends on no later token, whatever that holds.  Any strides with a contiguous
-    head dim are read in place if rows start on 16-byte boundaries."""
+    A token's output depends on no later token, whatever that holds.  From a token with an Inf or NaN on, the
+    states and outputs of its heads are not finite, NaN also where the definition has an infinity.  Any strides
+    with a contiguous head dim are read in place if rows start on 16-byte boundaries.  At most
+    2^20 - 16 sequences times heads.
+
+    Sums and states are float32.  float32 operands are used with all their 24 bits.  For bfloat16 the scores times
+    decays, and every 64 tokens the copy of the state that queries multiply, are rounded to bfloat16 once on the way, in the
+    backward too: o, d_q, d_k and d_v are 2.35e-3 from the definition as a whole, where rounding them alone is
+    1.66e-3.  With ``return_state`` (or a gradient to ``initial_state``) the state is updated with 24 bits of
+    the decayed values, without it with 16, which can show in the last bit of o."""
     name = "decay_attention"
     H, Hk, dk, dv = _check_qkv(name, q, k, v, log_gamma, 2)
     n_seq = q.shape[0]
@@ -236,7 +244,8 @@ def decay_attention_step(q, k, v, log_gamma, state, slots=None, scale: float | N
     """One token for each row: q, k [B, Hk, dk], v [B, H, dv] -> o [B, H, dv].  ``state`` [n, H, dk, dv]
     float32 is the cache of states, advanced in place; row b goes on from state ``slots[b]`` (int32 on the
     device; b without ``slots``).  Rows of one slot are consecutive tokens in the rows' order; a row whose slot
-    is outside [0, n) is padding, its output is zeros.  Records no gradient."""
+    is outside [0, n) is padding, its output is zeros.  At most 2^20 - 16 rows times heads.  float32 arithmetic.
+    Records no gradient."""
     name = "decay_attention_step"
     H, Hk, dk, dv = _check_qkv(name, q, k, v, log_gamma, 1)
     if state.dtype != torch.float32 or state.dim() != 4 or state.shape[1:] != (H, dk, dv):
@@ -262,7 +271,9 @@ def decay_attention_step(q, k, v, log_gamma, state, slots=None, scale: float | N
     _check_device(name, dev, k=k, v=v, log_gamma=log_gamma, state=state, slots=slots)
     if not (q.stride(-1) == k.stride(-1) == v.stride(-1) == 1):
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    if slots is not None and not slots.is_contiguous():
+        slots = slots.contiguous()
     o = on_device(dev, _step, q, k, v, _decays(log_gamma), dk ** -0.5 if scale is None else float(scale), state,
-                  slot_stride, slots if slots is None or slots.is_contiguous() else slots.contiguous(), (B, n, H, Hk, dk, dv, _DTYPES[q.dtype]))
+                  slot_stride, slots, (B, n, H, Hk, dk, dv, _DTYPES[q.dtype]))
     torch.autograd.graph.increment_version(state)
     return o

@@ -75,7 +75,8 @@ def group_norm(x, num_groups: int, weight=None, bias=None, gate=None, activation
     at most 1024, each to mean 0 and variance 1 (fp32), times ``weight`` [C] plus ``bias`` [C] (x's dtype
     or float32), then ``activation`` ("none", "silu" or "gelu", the exact one).  With ``gate`` (x's
     shape) the activation is of the gate and multiplies: norm(x) * act(gate).  Rows do not mix, so a
-    token's result does not depend on other tokens.  Differentiable in x, weight, bias and gate, once and in
+    token's result does not depend on other tokens.  fp32 arithmetic; bfloat16's silu uses the approximate
+    exponential and reciprocal, below its rounding.  Differentiable in x, weight, bias and gate, once and in
     reverse mode."""
     if x.dtype not in _DTYPES:
         raise TypeError(f"ttc_b200 group_norm supports float32 and bfloat16, got {x.dtype}")
