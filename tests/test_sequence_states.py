@@ -39,7 +39,8 @@ def test_a_timeout_belongs_to_its_device(monkeypatch):
     import ttc_b200
     m = sys.modules["ttc_b200.decay_attention"]
     words = [torch.zeros(1, dtype=torch.int32) for _ in range(2)]
-    monkeypatch.setattr(m, "_status", {i: (w, ctypes.c_int.from_address(w.data_ptr())) for i, w in enumerate(words)})
+    monkeypatch.setattr(m, "_status", {i: (w, ctypes.c_int.from_address(w.data_ptr()), w.data_ptr())
+                                       for i, w in enumerate(words)})
     synced = []
     monkeypatch.setattr(torch.cuda, "synchronize", synced.append)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)

@@ -27,9 +27,9 @@ def _workspace(nbytes: int, dev) -> torch.Tensor | None:
     return torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
 
 
-# For each device one word of pinned host memory that its kernels can reach, and a view of it: it is read at
-# the next call without waiting for the GPU.
-_status: dict[int, tuple[torch.Tensor, ctypes.c_int]] = {}
+# For each device one word of pinned host memory that its kernels can reach, a view of it and its address: it is
+# read at the next call without waiting for the GPU.
+_status: dict[int, tuple[torch.Tensor, ctypes.c_int, int]] = {}
 
 WAIT_TIMEOUT_MSG = ("ttc_b200 decay_attention: a wait inside an earlier call's kernel ran out "
                     "(that call's results are not valid)")
@@ -46,11 +46,14 @@ def _raise_timeout(device: int) -> None:
 def _status_word(device: int | None = None) -> int:
     """The address of the device's status word (None: of the current device's); raises as `_raise_timeout`."""
     device = torch.cuda.current_device() if device is None else device
-    if device not in _status:
+    held = _status.get(device)
+    if held is None:
         word = torch.zeros(1, dtype=torch.int32, device="cpu", pin_memory=True)
-        _status.setdefault(device, (word, ctypes.c_int.from_address(word.data_ptr())))
-    _raise_timeout(device)
-    return _status[device][0].data_ptr()
+        at = word.data_ptr()
+        held = _status.setdefault(device, (word, ctypes.c_int.from_address(at), at))
+    if held[1].value:
+        _raise_timeout(device)
+    return held[2]
 
 
 def check_decay_attention(device=None) -> None:
@@ -79,9 +82,12 @@ _SIX, _NINE = ctypes.c_int64 * 6, ctypes.c_int64 * 9
 
 
 def _strides(t: torch.Tensor):
-    """Strides of the dims before the head dim, 0 where none is taken: those of a dim of one element, and all of a
-    tensor of none, may be anything, in a contiguous tensor too, and the C entries want multiples of 16 bytes."""
-    return [s if n > 1 else 0 for n, s in zip(t.shape[:-1], t.stride())] if t.numel() else [0] * (t.dim() - 1)
+    """Strides of the dims before the head dim of t [B, T, heads, D], as the C entries want them: multiples of 16 bytes.
+    Those of a dim of one element, and all of an empty tensor, may be anything, in a contiguous tensor too."""
+    if t.is_contiguous():
+        _, T, H, D = t.shape
+        return T * H * D, H * D, D
+    return [s if n > 1 else 0 for n, s in zip(t.shape[:-1], t.stride())]
 
 
 def _check_qkv(name, q, k, v, log_gamma, lead):
@@ -227,7 +233,8 @@ def decay_attention(q, k, v, log_gamma, scale: float | None = None, initial_stat
                                       or tuple(initial_state.shape) != (n_seq, H, dk, dv)):
         raise ValueError(f"ttc_b200 {name}: initial_state must be float32 [{n_seq},{H},{dk},{dv}], got "
                          f"{initial_state.dtype} {tuple(initial_state.shape)}")
-    refuse_gradient(name, scale=scale)
+    if isinstance(scale, torch.Tensor):
+        refuse_gradient(name, scale=scale)
     refuse_tangents(name, q=q, k=k, v=v, log_gamma=log_gamma, initial_state=initial_state)
     _check_device(name, q.device, k=k, v=v, log_gamma=log_gamma, initial_state=initial_state, cu_seqlens=cu_seqlens)
     args = (_operand(q), _operand(k), _operand(v), _decays(log_gamma),
@@ -265,7 +272,8 @@ def decay_attention_step(q, k, v, log_gamma, state, slots=None, scale: float | N
         raise ValueError(f"ttc_b200 {name}: {B} rows and {n} states")
     if (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad) and torch.is_grad_enabled():
         raise ValueError(f"ttc_b200 {name} records no gradient: call it under torch.no_grad()")
-    refuse_gradient(name, scale=scale)
+    if isinstance(scale, torch.Tensor):
+        refuse_gradient(name, scale=scale)
     refuse_tangents(name, q=q, k=k, v=v, log_gamma=log_gamma, state=state)
     dev = q.device
     _check_device(name, dev, k=k, v=v, log_gamma=log_gamma, state=state, slots=slots)

@@ -92,7 +92,8 @@ def group_norm(x, num_groups: int, weight=None, bias=None, gate=None, activation
     for p in params:
         if p.shape != (C,) or p.dtype not in (x.dtype, torch.float32) or p.dtype != params[0].dtype:
             raise ValueError(f"ttc_b200 group_norm: weight and bias must be [{C}] in {x.dtype} or both float32")
-    refuse_gradient("group_norm", eps=eps)
+    if isinstance(eps, torch.Tensor):
+        refuse_gradient("group_norm", eps=eps)
     refuse_tangents("group_norm", x=x, weight=weight, bias=bias, gate=gate)
     dev = x.device
     for t, n in ((weight, "weight"), (bias, "bias"), (gate, "gate")):

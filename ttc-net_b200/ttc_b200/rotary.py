@@ -125,8 +125,9 @@ def rotary(q, k, positions, inv_freq, interleaved: bool = False, magnitude: floa
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or 2 * inv_freq.numel() > D:
         raise ValueError(f"ttc_b200 rotary: inv_freq must be float64 [R / 2] with R <= {D}, got "
                          f"{inv_freq.dtype} {tuple(inv_freq.shape)}")
-    refuse_gradient("rotary", inv_freq=inv_freq, magnitude=magnitude)
-    refuse_tangents("rotary", q=q, k=k)
+    if inv_freq.requires_grad or isinstance(magnitude, torch.Tensor):
+        refuse_gradient("rotary", inv_freq=inv_freq, magnitude=magnitude)
+    refuse_tangents("rotary", q=q, k=k, inv_freq=inv_freq)
     dev = q.device
     for t, n in ((k, "k"), (positions, "positions"), (inv_freq, "inv_freq")):
         if t is not None and t.device != dev:
