@@ -209,3 +209,60 @@ def test_many_rows_behind_the_last_sequence(H, Hk, dk, dv, T, dtype):
     del stale  # what the outputs are allocated from
     for a, b in zip(call(ins, go), want):
         assert torch.equal(a[:, :50], b) and (a[:, 50:] == 0).all()
+
+
+def _room(gb):
+    if torch.cuda.mem_get_info()[0] < gb << 30:
+        pytest.skip(f"needs {gb} GB")
+
+
+def test_gradients_of_more_than_2_31_values():
+    """The last tokens of 2^20 against a short call: of decays by e^-1/8 a token, what is 4096 tokens away weighs e^-512."""
+    from ttc_b200 import decay_attention
+    _room(48)
+    T, H = 1 << 20, 17
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, k = (torch.randn(1, T, H, 8, generator=g, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    v, go = (torch.randn(1, T, H, 128, generator=g, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    assert v.numel() > 1 << 31
+    lg, res = torch.full((H,), -0.125, device="cuda"), []
+    for n in (T, 8192):
+        ins = [t[:, -n:].detach().requires_grad_() for t in (q, k, v)]
+        res.append([t[:, -4096:].float() for t in torch.autograd.grad(decay_attention(*ins, lg), ins, go[:, -n:])])
+    for a, b in zip(*res):
+        assert ((a - b).abs() <= 2.0 ** -7 * (b.abs() + b.abs().max())).all()
+
+
+def test_rotary_of_more_than_2_31_values():
+    from ttc_b200 import rotary, rotary_frequencies
+    _room(24)
+    T, H, D = (1 << 17) + 3, 129, 128
+    q = torch.randn(1, T, H, D, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    assert q.numel() > 1 << 31
+    f, _ = rotary_frequencies(64)
+    pos = torch.arange(T, device="cuda")
+    tail = q.detach()[:, -50:].requires_grad_()
+    y, _ = rotary(q, None, pos, f)
+    z, _ = rotary(tail, None, pos[-50:], f)
+    assert torch.equal(y[:, -50:], z)
+    a, = torch.autograd.grad(y, q, y.detach())
+    b, = torch.autograd.grad(z, tail, z.detach())
+    assert torch.equal(a[:, -50:], b)
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+def test_group_norm_of_more_than_2_31_values(shift):
+    """With 16-byte accesses, and one value at a time (rows off the 16-byte grid)."""
+    from ttc_b200 import group_norm
+    _room(40)
+    rows, groups, n = (1 << 17) + 5, 41, 400
+    C = groups * n
+    x = torch.randn(rows * C + 1, device="cuda", dtype=torch.bfloat16)[shift:shift + rows * C].view(rows, C).requires_grad_()
+    assert x.numel() > 1 << 31
+    w = _normal(3, C, dtype=torch.bfloat16)
+    tail = torch.empty(20 * C + 1, device="cuda", dtype=torch.bfloat16)[shift:shift + 20 * C].view(20, C).copy_(x.detach()[-20:]).requires_grad_()
+    y, z = (group_norm(t, groups, w, activation="silu") for t in (x, tail))
+    assert torch.equal(y[-20:], z)
+    a, = torch.autograd.grad(y, x, y.detach())
+    b, = torch.autograd.grad(z, tail, z.detach())
+    assert torch.equal(a[-20:], b)
