@@ -217,7 +217,8 @@ struct Plan {
 // How a call is split: one CTA for each (sequence, head, pass), or sequences cut into segments whose states
 // are summed first (a second pass over k and v) and joined by a scan.  The least cost over the number of segments decides,
 // segments have at least four blocks.  In units of a block's time on one CTA (1.9 us in bf16 at 128 x 128, 1.5 at
-// 64 x 64; in fp32 7 us at 32 x 64, 9 at 64 x 64; one set of costs for all widths), `rounds` of CTAs over the SMs cost their segment's blocks and
+// 64 x 64; in fp32 7 us at 32 x 64, 9 at 64 x 64; one set of costs for all
+// widths), `rounds` of CTAs over the SMs cost their segment's blocks and
 // `start` for a CTA's beginning and end; those of the sums `sum` of the blocks and `sum_start`; `more` is for the two
 // further launches, `state` for the trips of one segment's 128 x 128 state through memory.  Fitted to measured times: 8192
 // tokens, 32 heads of 128: 224 us as one, 134 in 4 segments, 187 in 9; 2 x 4096: 116 as one, 129 in 2.  A backward counts as one

@@ -144,8 +144,8 @@ __device__ __forceinline__ float decay_pow(float lg, int64_t n) {
 
 // Zeros in the rows behind the last packed sequence.  Over all heads they are one range of memory: each of the CTAs
 // that a launch has for it (clearing_ctas for each head) takes an equal share of every stretch of it, 16 bytes a
-// thread (vd is a multiple of 8 and the outputs start on 16-byte boundaries).  A row of 32 768
-// tokens, 32 heads of 128 bf16, with 2 000 in use: the call takes 71 us; with one CTA a head, row after row, 4 840.
+// thread (vd is a multiple of 8 and the outputs start on 16-byte boundaries).  A row of 32 768 tokens, 32 heads of 128
+// bf16, with 2 000 in use: the call takes 71 us; with one CTA a head, row after row, 4 840.
 template <bool BF16>
 __device__ __forceinline__ void zero_rows_behind(const Args& A, const Pass& P, int h, int tid, int threads) {
   int64_t row0, len;

@@ -31,7 +31,7 @@ def on_device(dev, f, *args):
 def refuse_tangents(name, **operands) -> None:
     """Raises where an operand carries a forward-mode tangent.  The kernels write into new tensors, which
     have none, and a dual tensor need not require a gradient: the result would pass for a constant."""
-    # the number of the innermost dual level, negative outside of all (a call costs 0.2 us there)
+    # the number of the innermost dual level, negative outside of all (this costs 0.13 us there)
     if forward_ad._current_level < 0 or not torch._C._is_fwd_grad_enabled():
         return
     for n, t in operands.items():

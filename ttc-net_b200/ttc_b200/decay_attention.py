@@ -210,15 +210,15 @@ def decay_attention(q, k, v, log_gamma, scale: float | None = None, initial_stat
     sequence i the tokens cu_seqlens[i] .. cu_seqlens[i + 1] - 1; states are [n, H, dk, dv].  Rows
     behind the last sequence get zeros.  Offsets past the row are cut to it.
 
-    A token's output depends on no later token, whatever that holds.  From a token with an Inf or NaN on, the
-    states and outputs of its heads are not finite, NaN also where the definition has an infinity.  Any strides
-    with a contiguous head dim are read in place if rows start on 16-byte boundaries.  At most
+    A token's output depends on no later token, whatever that holds.  What an Inf or NaN in k or v
+    reaches, later outputs and states of its heads, is not finite, and NaN also where the definition has an infinity.
+    Any strides with a contiguous head dim are read in place if rows start on 16-byte boundaries.  At most
     2^20 - 16 sequences times heads.
 
     Sums and states are float32.  float32 operands are used with all their 24 bits.  For bfloat16 the scores times
     decays, and every 64 tokens the copy of the state that queries multiply, are rounded to bfloat16 once on the way, in the
-    backward too: o, d_q, d_k and d_v are 2.35e-3 from the definition as a whole, where rounding them alone is
-    1.66e-3.  With ``return_state`` (or a gradient to ``initial_state``) the state is updated with 24 bits of
+    backward too: for random operands o, d_q, d_k and d_v are 2.35e-3 from the definition as a whole, where rounding
+    them alone is 1.66e-3.  With ``return_state`` (or a gradient to ``initial_state``) the state is updated with 24 bits of
     the decayed values, without it with 16, which can show in the last bit of o."""
     name = "decay_attention"
     H, Hk, dk, dv = _check_qkv(name, q, k, v, log_gamma, 2)
